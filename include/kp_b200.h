@@ -29,6 +29,7 @@ extern "C" {
 #define KPB_F32 0
 #define KPB_F16 1
 #define KPB_BF16 2
+#define KPB_E4M3 3 /* cache element type only: 8-bit codes with one fp32 scale per row */
 
 /* status codes */
 #define KPB_OK 0
@@ -43,14 +44,17 @@ const char* kpb_last_error(void);
 int kpb_version(void);
 
 /* Number of variants of an op ("vector_add", "reduce_sum", "softmax", "matmul",
- * "layernorm", "attention", "attention_causal"), or -1 for an unknown name. Mirrors
- * check_variant's counts (csrc/bindings.cpp:30-33, :77, :111). */
+ * "layernorm", "attention", "attention_causal", "qk_norm_rope",
+ * "qk_norm_rope_backward", "kv_cache_write", "kv_cache_read", "paged_attention"), or -1
+ * for an unknown name. Mirrors check_variant's counts (csrc/bindings.cpp:30-33, :77,
+ * :111). */
 int kpb_num_variants(const char* op);
 
 /* Error bits that kernels on the current device recorded since the last call
- * (bit 0 = a bounded wait inside a kernel gave up), then cleared. No counterpart in
- * the reference, whose kernels have no waits. Synchronous; for tests and health
- * checks, not hot paths. */
+ * (bit 0 = a bounded wait inside a kernel gave up, bit 2 = a slot, page, position or
+ * length outside its table), then cleared. No counterpart in the reference, whose
+ * kernels have no waits and no index tables. Synchronous; for tests and health checks,
+ * not hot paths. */
 int kpb_device_errors(unsigned* bits);
 
 /* ---- elementwise add: replaces kp::vector_add (csrc/launchers.h:12-13) ----
@@ -150,6 +154,90 @@ int kpb_attention(int variant, int dtype, const void* q, const void* k, const vo
 int kpb_attention_causal(int variant, int dtype, const void* q, const void* k,
                          const void* v, void* o, int64_t BH, int64_t S, int64_t D,
                          void* stream);
+
+/* ======================================================================
+ * The decode step: new operators, no counterpart in the reference.
+ * Indices are read on the device and checked there: one outside its table is never
+ * followed; the affected rows become NaN (nothing is written for a cache write) and bit 2
+ * of kpb_device_errors() is set. Calls run on the current device, which must hold every
+ * pointer. D <= 256.
+ * ====================================================================== */
+
+/* ---- RMS norm of query and key heads with the position rotation ----
+ * For every token t < T and head: y = x / sqrt(mean(x^2) + eps) * weight over the D
+ * elements, then the first `rot` (even, <= D) elements turned in pairs by the angles of
+ * positions[t]: (a, b) -> (a cos - b sin, b cos + a sin), pairs (i, i + rot/2), or
+ * (2i, 2i + 1) if `interleaved`. cos_sin is fp32 (max_pos, rot): rot/2 cosines then rot/2
+ * sines per position. q is (T, Hq, D) and k (T, Hkv, D), the heads of a token contiguous
+ * and tokens q_stride / k_stride elements apart (slices of a fused projection); q_out and
+ * k_out are contiguous. fp32 until one rounding to the dtype. */
+int kpb_qk_norm_rope(int variant, int dtype, const void* q, const void* k, const void* q_weight,
+                     const void* k_weight, const float* cos_sin, const int64_t* positions,
+                     void* q_out, void* k_out, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                     int64_t rot, int64_t max_pos, int64_t q_stride, int64_t k_stride, float eps,
+                     int interleaved, void* stream);
+
+/* Its gradient: from grad_q, grad_k (the gradients of q_out, k_out) and the forward's
+ * inputs, dq (T, Hq, D), dk (T, Hkv, D) contiguous and dq_weight, dk_weight (D), every one
+ * overwritten. The weight gradients are summed over all rows in fp32 in a fixed order (the
+ * same bits every time on one kind of GPU). workspace: kpb_qk_norm_rope_backward_
+ * workspace_bytes() bytes, 16-byte aligned, the call's own until it has run. */
+size_t kpb_qk_norm_rope_backward_workspace_bytes(int64_t T, int64_t Hq, int64_t Hkv, int64_t D);
+int kpb_qk_norm_rope_backward(int variant, int dtype, const void* grad_q, const void* grad_k,
+                              const void* q, const void* k, const void* q_weight,
+                              const void* k_weight, const float* cos_sin,
+                              const int64_t* positions, void* dq, void* dk, void* dq_weight,
+                              void* dk_weight, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                              int64_t rot, int64_t max_pos, int64_t grad_q_stride,
+                              int64_t grad_k_stride, int64_t q_stride, int64_t k_stride,
+                              float eps, int interleaved, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* ---- paged key/value cache ----
+ * k_cache and v_cache are (num_pages, Hkv, page_size, D), each page's inner part
+ * contiguous, pages page_stride >= Hkv * page_size * D elements apart (the same for both),
+ * of type cache_dtype: the call's dtype, or KPB_E4M3 with fp32 scales k_scale, v_scale,
+ * contiguous (num_pages, Hkv, page_size). A slot is page * page_size + offset.
+ *
+ * write: row (t, h) of k and v (heads of a token contiguous, tokens k_stride / v_stride
+ * elements apart) to slot slots[t]; slots below 0 are skipped; nothing else of the caches
+ * changes. E4M3: the scale is the smallest power of two (>= 2^-126) that brings the row's
+ * largest magnitude to at most 448 (1 for a row of zeros), and a code is x / scale rounded
+ * to nearest even; a row holding an infinity or NaN gets the scale NaN and zero codes.
+ * Slots of one call must differ: of two tokens with one slot, either's elements may stay.
+ *
+ * read: k and v (T, Hkv, D) contiguous in `dtype` from slots[t]; E4M3 rows as code * scale
+ * rounded once; rows of slots below 0 are zeros. Any scales may be read, not only powers
+ * of two. */
+int kpb_kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, const void* v,
+                       const int64_t* slots, void* k_cache, void* v_cache, float* k_scale,
+                       float* v_scale, int64_t T, int64_t Hkv, int64_t D, int64_t num_pages,
+                       int64_t page_size, int64_t k_stride, int64_t v_stride,
+                       int64_t page_stride, void* stream);
+int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cache,
+                      const void* v_cache, const int64_t* slots, const float* k_scale,
+                      const float* v_scale, void* k, void* v, int64_t T, int64_t Hkv, int64_t D,
+                      int64_t num_pages, int64_t page_size, int64_t page_stride, void* stream);
+
+/* ---- attention of one new token per sequence over the paged cache ----
+ * o[b, h] = softmax_j(scale * q[b, h] . K[j]) V[j] for j < seq_lens[b], K[j] and V[j] the
+ * rows of key head h / (Hq / Hkv) in page block_table[b * table_stride + j / page_size] at
+ * offset j % page_size of the cache above. q is (B, Hq, D) with sequences q_stride
+ * elements apart, o contiguous; Hq a multiple of Hkv. seq_lens[b] = 0 gives zeros. Cache
+ * rows past a sequence's last key and table entries past its last page are not read.
+ * E4M3 scales must not be negative, and codes must not be NaN (a cache written by
+ * kpb_kv_cache_write has neither).
+ * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size),
+ * 16-byte aligned, the call's own until it has run. */
+size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,
+                                           int64_t D, int64_t max_len);
+int kpb_paged_attention(int variant, int dtype, int cache_dtype, const void* q,
+                        const void* k_cache, const void* v_cache, const int* block_table,
+                        const int* seq_lens, const float* k_scale, const float* v_scale, void* o,
+                        int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
+                        int64_t page_size, int64_t max_pages, int64_t q_stride,
+                        int64_t page_stride, int64_t table_stride, float scale, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

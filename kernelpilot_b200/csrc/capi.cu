@@ -7,6 +7,7 @@
 #include <tuple>
 
 #include "kp_common.cuh"
+#include "kp_kv_cache.cuh"
 
 namespace kpb {
 
@@ -25,6 +26,36 @@ int layernorm(int variant, int dtype, const void* x, const void* w, const void* 
               int64_t M, int64_t N, float eps, cudaStream_t s);
 int attention(int variant, int dtype, bool causal, const void* q, const void* k, const void* v,
               void* o, int64_t BH, int64_t S, int64_t D, unsigned* err, cudaStream_t s);
+int qk_norm_rope(int variant, int dtype, const void* q, const void* k, const void* wq,
+                 const void* wk, const float* cos_sin, const int64_t* positions, void* q_out,
+                 void* k_out, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim,
+                 int64_t rot, int64_t max_pos, int64_t q_stride, int64_t k_stride, float eps,
+                 bool interleaved, unsigned* err, cudaStream_t s);
+size_t qk_norm_rope_backward_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t k_heads,
+                                             int64_t dim);
+int qk_norm_rope_backward(int variant, int dtype, const void* gq, const void* gk, const void* q,
+                          const void* k, const void* wq, const void* wk, const float* cos_sin,
+                          const int64_t* positions, void* dq, void* dk, void* dwq, void* dwk,
+                          int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim,
+                          int64_t rot, int64_t max_pos, int64_t gq_stride, int64_t gk_stride,
+                          int64_t q_stride, int64_t k_stride, float eps, bool interleaved,
+                          void* ws, unsigned* err, cudaStream_t s);
+int kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, const void* v,
+                   const int64_t* slots, void* k_cache, void* v_cache, float* k_scale,
+                   float* v_scale, int64_t tokens, int64_t k_stride, int64_t v_stride,
+                   const KvLayout& lay, unsigned* err, cudaStream_t s);
+int kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cache,
+                  const void* v_cache, const int64_t* slots, const float* k_scale,
+                  const float* v_scale, void* k, void* v, int64_t tokens, const KvLayout& lay,
+                  unsigned* err, cudaStream_t s);
+size_t paged_attention_workspace_bytes(int variant, int64_t batch, int64_t q_heads,
+                                       int64_t k_heads, int64_t dim, int64_t max_len);
+int paged_attention(int variant, int dtype, int cache_dtype, const void* q, const void* k_cache,
+                    const void* v_cache, const int* table, const int* seq_lens,
+                    const float* k_scale, const float* v_scale, void* o, int64_t batch,
+                    int64_t q_heads, int64_t max_pages, int64_t q_stride, int64_t table_stride,
+                    float scale, const KvLayout& lay, void* ws, size_t ws_bytes, unsigned* err,
+                    cudaStream_t s);
 
 namespace {
 thread_local std::string g_last_error;
@@ -192,6 +223,58 @@ static int check_common(const char* op, int variant, int dtype) {
 
 static size_t elem_bytes(int dtype) { return dtype == KPB_F32 ? 4 : 2; }
 
+constexpr int64_t kSizeLimit = int64_t{1} << 31;
+
+static bool size_ok(int64_t n) { return n >= 0 && n < kSizeLimit; }
+
+static bool off_by(const void* p, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes != 0;
+}
+
+// Sizes of qk_norm_rope and its backward.
+static int check_rope(const std::string& op, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                      int64_t rot, int64_t max_pos) {
+  if (!size_ok(T) || !size_ok(Hq) || !size_ok(Hkv) || !size_ok(max_pos) ||
+      !size_ok(T * (Hq + Hkv)))
+    return fail(KPB_EINVAL, op + ": T, heads, T * heads and max_pos must be in [0, 2^31)");
+  if (D < 1 || D > kMaxHeadDim) return fail(KPB_EINVAL, op + ": D must be in [1, 256]");
+  if (rot < 0 || rot > D || rot % 2 != 0)
+    return fail(KPB_EINVAL, op + ": rot must be even and in [0, D]");
+  return KPB_OK;
+}
+
+// Sizes, types and strides of a paged cache.
+static int check_cache(const std::string& op, int dtype, int cache_dtype, const void* k_cache,
+                       const void* v_cache, const void* k_scale, const void* v_scale,
+                       const KvLayout& lay) {
+  if (cache_dtype != dtype && cache_dtype != KPB_E4M3)
+    return fail(KPB_EINVAL, op + ": cache dtype must be the call's dtype or 3 (e4m3)");
+  if (!size_ok(lay.num_pages) || !size_ok(lay.page_size) || lay.page_size < 1 ||
+      !size_ok(lay.heads))
+    return fail(KPB_EINVAL,
+                op + ": num_pages and Hkv must be in [0, 2^31), page_size in [1, 2^31)");
+  if (lay.dim < 1 || lay.dim > kMaxHeadDim)
+    return fail(KPB_EINVAL, op + ": D must be in [1, 256]");
+  if (!size_ok(lay.heads * lay.page_size))
+    return fail(KPB_EINVAL, op + ": Hkv * page_size must be below 2^31");
+  if (lay.num_pages > 1 && lay.page_stride < lay.heads * lay.page_size * lay.dim)
+    return fail(KPB_EINVAL, op + ": page_stride is shorter than a page");
+  if (lay.num_pages > 0 && lay.page_stride > INT64_MAX / 16 / lay.num_pages)
+    return fail(KPB_EINVAL, op + ": the cache is too large");
+  const bool any = lay.num_pages > 0 && lay.heads > 0;
+  if (any && (k_cache == nullptr || v_cache == nullptr))
+    return fail(KPB_EINVAL, op + ": null pointer");
+  if (cache_dtype == KPB_E4M3) {
+    if (any && (k_scale == nullptr || v_scale == nullptr))
+      return fail(KPB_EINVAL, op + ": an e4m3 cache needs k_scale and v_scale (null pointer)");
+    if (off_by(k_scale, 4) || off_by(v_scale, 4))
+      return fail(KPB_EINVAL, op + ": scales must be element-aligned");
+  } else if (off_by(k_cache, elem_bytes(dtype)) || off_by(v_cache, elem_bytes(dtype))) {
+    return fail(KPB_EINVAL, op + ": tensors must be element-aligned");
+  }
+  return KPB_OK;
+}
+
 }  // namespace kpb
 
 using namespace kpb;
@@ -208,6 +291,9 @@ int kpb_num_variants(const char* op) {
   if (s == "vector_add" || s == "reduce_sum" || s == "softmax" || s == "layernorm") return 3;
   if (s == "matmul") return 4;
   if (s == "attention" || s == "attention_causal") return 2;
+  if (s == "qk_norm_rope" || s == "qk_norm_rope_backward" || s == "kv_cache_write" ||
+      s == "kv_cache_read" || s == "paged_attention")
+    return 2;
   return -1;
 }
 
@@ -360,6 +446,178 @@ int kpb_attention(int variant, int dtype, const void* q, const void* k, const vo
 int kpb_attention_causal(int variant, int dtype, const void* q, const void* k, const void* v,
                          void* o, int64_t BH, int64_t S, int64_t D, void* stream) {
   return attention_entry("attention_causal", true, variant, dtype, q, k, v, o, BH, S, D, stream);
+}
+
+int kpb_qk_norm_rope(int variant, int dtype, const void* q, const void* k, const void* q_weight,
+                     const void* k_weight, const float* cos_sin, const int64_t* positions,
+                     void* q_out, void* k_out, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                     int64_t rot, int64_t max_pos, int64_t q_stride, int64_t k_stride, float eps,
+                     int interleaved, void* stream) {
+  g_last_error.clear();
+  if (int rc = check_common("qk_norm_rope", variant, dtype)) return rc;
+  if (int rc = check_rope("qk_norm_rope", T, Hq, Hkv, D, rot, max_pos)) return rc;
+  if (T == 0 || Hq + Hkv == 0) return KPB_OK;
+  if (positions == nullptr || (rot > 0 && max_pos > 0 && cos_sin == nullptr) ||
+      (Hq > 0 && (!q || !q_weight || !q_out)) || (Hkv > 0 && (!k || !k_weight || !k_out)))
+    return fail(KPB_EINVAL, "qk_norm_rope: null pointer");
+  const size_t es = elem_bytes(dtype);
+  if (off_by(q, es) || off_by(k, es) || off_by(q_weight, es) || off_by(k_weight, es) ||
+      off_by(q_out, es) || off_by(k_out, es) || off_by(cos_sin, 4) || off_by(positions, 8))
+    return fail(KPB_EINVAL, "qk_norm_rope: tensors must be element-aligned");
+  unsigned* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  return qk_norm_rope(variant, dtype, q, k, q_weight, k_weight, cos_sin, positions, q_out, k_out,
+                      T, Hq, Hkv, D, rot, max_pos, q_stride, k_stride, eps, interleaved != 0, err,
+                      static_cast<cudaStream_t>(stream));
+}
+
+size_t kpb_qk_norm_rope_backward_workspace_bytes(int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (check_rope("qk_norm_rope_backward", T, Hq, Hkv, D, 0, 0) != KPB_OK) return 0;
+  return qk_norm_rope_backward_workspace_bytes(T, Hq, Hkv, D);
+}
+
+int kpb_qk_norm_rope_backward(int variant, int dtype, const void* grad_q, const void* grad_k,
+                              const void* q, const void* k, const void* q_weight,
+                              const void* k_weight, const float* cos_sin,
+                              const int64_t* positions, void* dq, void* dk, void* dq_weight,
+                              void* dk_weight, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                              int64_t rot, int64_t max_pos, int64_t grad_q_stride,
+                              int64_t grad_k_stride, int64_t q_stride, int64_t k_stride,
+                              float eps, int interleaved, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  const char* op = "qk_norm_rope_backward";
+  if (int rc = check_common(op, variant, dtype)) return rc;
+  if (int rc = check_rope(op, T, Hq, Hkv, D, rot, max_pos)) return rc;
+  const std::string name(op);
+  if (!dq_weight || !dk_weight || (T > 0 && !positions) ||
+      (T > 0 && rot > 0 && max_pos > 0 && cos_sin == nullptr) ||
+      (T * Hq > 0 && (!grad_q || !q || !q_weight || !dq)) ||
+      (T * Hkv > 0 && (!grad_k || !k || !k_weight || !dk)))
+    return fail(KPB_EINVAL, name + ": null pointer");
+  const size_t es = elem_bytes(dtype);
+  const void* ptrs[10] = {grad_q, grad_k, q, k, q_weight, k_weight, dq, dk, dq_weight, dk_weight};
+  for (const void* p : ptrs)
+    if (off_by(p, es)) return fail(KPB_EINVAL, name + ": tensors must be element-aligned");
+  if (off_by(cos_sin, 4) || off_by(positions, 8))
+    return fail(KPB_EINVAL, name + ": tensors must be element-aligned");
+  const size_t need = qk_norm_rope_backward_workspace_bytes(T, Hq, Hkv, D);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(KPB_EINVAL, name + ": workspace too small (" + std::to_string(workspace_bytes) +
+                                " bytes, need " + std::to_string(need) + ")");
+  if (off_by(workspace, 16)) return fail(KPB_EINVAL, name + ": workspace must be 16-byte aligned");
+  unsigned* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  return qk_norm_rope_backward(variant, dtype, grad_q, grad_k, q, k, q_weight, k_weight, cos_sin,
+                               positions, dq, dk, dq_weight, dk_weight, T, Hq, Hkv, D, rot,
+                               max_pos, grad_q_stride, grad_k_stride, q_stride, k_stride, eps,
+                               interleaved != 0, workspace, err,
+                               static_cast<cudaStream_t>(stream));
+}
+
+int kpb_kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, const void* v,
+                       const int64_t* slots, void* k_cache, void* v_cache, float* k_scale,
+                       float* v_scale, int64_t T, int64_t Hkv, int64_t D, int64_t num_pages,
+                       int64_t page_size, int64_t k_stride, int64_t v_stride,
+                       int64_t page_stride, void* stream) {
+  g_last_error.clear();
+  const char* op = "kv_cache_write";
+  const KvLayout lay{num_pages, page_size, Hkv, D, page_stride};
+  if (int rc = check_common(op, variant, dtype)) return rc;
+  if (int rc = check_cache(op, dtype, cache_dtype, k_cache, v_cache, k_scale, v_scale, lay))
+    return rc;
+  if (!size_ok(T) || !size_ok(T * Hkv))
+    return fail(KPB_EINVAL, "kv_cache_write: T and T * Hkv must be in [0, 2^31)");
+  if (T == 0 || Hkv == 0) return KPB_OK;
+  if (!k || !v || !slots) return fail(KPB_EINVAL, "kv_cache_write: null pointer");
+  if (num_pages > 0 && k_cache == v_cache)
+    return fail(KPB_EINVAL, "kv_cache_write: k_cache and v_cache must differ");
+  if (off_by(k, elem_bytes(dtype)) || off_by(v, elem_bytes(dtype)) || off_by(slots, 8))
+    return fail(KPB_EINVAL, "kv_cache_write: tensors must be element-aligned");
+  unsigned* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  return kv_cache_write(variant, dtype, cache_dtype, k, v, slots, k_cache, v_cache, k_scale,
+                        v_scale, T, k_stride, v_stride, lay, err,
+                        static_cast<cudaStream_t>(stream));
+}
+
+int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cache,
+                      const void* v_cache, const int64_t* slots, const float* k_scale,
+                      const float* v_scale, void* k, void* v, int64_t T, int64_t Hkv, int64_t D,
+                      int64_t num_pages, int64_t page_size, int64_t page_stride, void* stream) {
+  g_last_error.clear();
+  const char* op = "kv_cache_read";
+  const KvLayout lay{num_pages, page_size, Hkv, D, page_stride};
+  if (int rc = check_common(op, variant, dtype)) return rc;
+  if (int rc = check_cache(op, dtype, cache_dtype, k_cache, v_cache, k_scale, v_scale, lay))
+    return rc;
+  if (!size_ok(T) || !size_ok(T * Hkv))
+    return fail(KPB_EINVAL, "kv_cache_read: T and T * Hkv must be in [0, 2^31)");
+  if (T == 0 || Hkv == 0) return KPB_OK;
+  if (!k || !v || !slots) return fail(KPB_EINVAL, "kv_cache_read: null pointer");
+  if (off_by(k, elem_bytes(dtype)) || off_by(v, elem_bytes(dtype)) || off_by(slots, 8))
+    return fail(KPB_EINVAL, "kv_cache_read: tensors must be element-aligned");
+  unsigned* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  return kv_cache_read(variant, dtype, cache_dtype, k_cache, v_cache, slots, k_scale, v_scale, k,
+                       v, T, lay, err, static_cast<cudaStream_t>(stream));
+}
+
+static int check_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  const std::string op("paged_attention");
+  if (!size_ok(B) || !size_ok(Hq) || !size_ok(Hkv) || !size_ok(B * Hq))
+    return fail(KPB_EINVAL, op + ": B, heads and B * Hq must be in [0, 2^31)");
+  if (Hq > 0 && (Hkv == 0 || Hq % Hkv != 0))
+    return fail(KPB_EINVAL, op + ": Hq must be a multiple of Hkv");
+  if (D < 1 || D > kMaxHeadDim) return fail(KPB_EINVAL, op + ": D must be in [1, 256]");
+  return KPB_OK;
+}
+
+size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,
+                                           int64_t D, int64_t max_len) {
+  if (variant < 0 || variant >= kpb_num_variants("paged_attention") || max_len < 0 ||
+      check_paged(B, Hq, Hkv, D) != KPB_OK || B == 0 || Hq == 0)
+    return 0;
+  return paged_attention_workspace_bytes(variant, B, Hq, Hkv, D, max_len);
+}
+
+int kpb_paged_attention(int variant, int dtype, int cache_dtype, const void* q,
+                        const void* k_cache, const void* v_cache, const int* block_table,
+                        const int* seq_lens, const float* k_scale, const float* v_scale, void* o,
+                        int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
+                        int64_t page_size, int64_t max_pages, int64_t q_stride,
+                        int64_t page_stride, int64_t table_stride, float scale, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  const char* op = "paged_attention";
+  const std::string name(op);
+  const KvLayout lay{num_pages, page_size, Hkv, D, page_stride};
+  if (int rc = check_common(op, variant, dtype)) return rc;
+  if (int rc = check_cache(op, dtype, cache_dtype, k_cache, v_cache, k_scale, v_scale, lay))
+    return rc;
+  if (int rc = check_paged(B, Hq, Hkv, D)) return rc;
+  if (!size_ok(max_pages) || !size_ok(max_pages * page_size))
+    return fail(KPB_EINVAL, name + ": max_pages * page_size must be in [0, 2^31)");
+  if (B == 0 || Hq == 0) return KPB_OK;
+  if (!q || !seq_lens || !o || (max_pages > 0 && !block_table))
+    return fail(KPB_EINVAL, name + ": null pointer");
+  if (off_by(q, elem_bytes(dtype)) || off_by(o, elem_bytes(dtype)) || off_by(block_table, 4) ||
+      off_by(seq_lens, 4))
+    return fail(KPB_EINVAL, name + ": tensors must be element-aligned");
+  const size_t need =
+      paged_attention_workspace_bytes(variant, B, Hq, Hkv, D, max_pages * page_size);
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(KPB_EINVAL, name + ": workspace too small (" + std::to_string(workspace_bytes) +
+                                  " bytes, need " + std::to_string(need) + ")");
+    if (off_by(workspace, 16))
+      return fail(KPB_EINVAL, name + ": workspace must be 16-byte aligned");
+  }
+  unsigned* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  return paged_attention(variant, dtype, cache_dtype, q, k_cache, v_cache, block_table, seq_lens,
+                         k_scale, v_scale, o, B, Hq, max_pages, q_stride, table_stride, scale,
+                         lay, workspace, workspace_bytes, err, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -83,9 +83,19 @@ CAPI_SIGNATURES: dict[str, tuple] = {
     "kpb_layernorm": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp]),
     "kpb_attention": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "kpb_attention_causal": (_i32, [_i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "kpb_qk_norm_rope": (_i32, [_i32, _i32, *[_vp] * 8, *[_i64] * 8, ctypes.c_float, _i32, _vp]),
+    "kpb_qk_norm_rope_backward_workspace_bytes": (_sz, [_i64] * 4),
+    "kpb_qk_norm_rope_backward": (_i32, [_i32, _i32, *[_vp] * 12, *[_i64] * 10, ctypes.c_float,
+                                         _i32, _vp, _sz, _vp]),
+    "kpb_kv_cache_write": (_i32, [_i32, _i32, _i32, *[_vp] * 7, *[_i64] * 8, _vp]),
+    "kpb_kv_cache_read": (_i32, [_i32, _i32, _i32, *[_vp] * 7, *[_i64] * 6, _vp]),
+    "kpb_paged_attention_workspace_bytes": (_sz, [_i32, *[_i64] * 5]),
+    "kpb_paged_attention": (_i32, [_i32, _i32, _i32, *[_vp] * 8, *[_i64] * 10, ctypes.c_float,
+                                   _vp, _sz, _vp]),
 }
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CACHE_DTYPE_CODES = {**DTYPE_CODES, torch.float8_e4m3fn: 3}
 
 
 @lru_cache(maxsize=1)

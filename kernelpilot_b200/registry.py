@@ -9,14 +9,20 @@ counts match the reference (3 / 3 / 3 / 4 / 3 / 2), so a caller passing the refe
 "best" variant index gets the B200 kernel. LayerNorm's eps goes between the inputs and
 the variant, as the reference's ``_HIP_EXTRA_ARGS`` (:28) passes it. Triton twins are not registered: the
 product path has no Triton dispatch.
+
+The decode step's operators (``DECODE_STAGES``) stand beside them under the same scheme;
+their contracts are in ``specs_decode.py``.
 """
 
 from __future__ import annotations
 
 from collections.abc import Callable
 
+import torch
+
 from . import ext
 from .specs import LAYERNORM_EPS, get_spec
+from .specs_decode import DECODE_SPECS, NORM_EPS
 
 CUDA_STAGES: dict[str, list[str]] = {
     "vector_add": ["naive", "gridstride", "vectorized"],
@@ -28,19 +34,39 @@ CUDA_STAGES: dict[str, list[str]] = {
     "attention_causal": ["naive", "tcgen05_flash"],
 }
 
-BEST_VARIANT: dict[str, int] = {k: len(v) - 1 for k, v in CUDA_STAGES.items()}
+DECODE_STAGES: dict[str, list[str]] = {
+    "qk_norm_rope": ["warp_row", "vector_pairs"],
+    "qk_norm_rope_backward": ["warp_row", "vector_pairs"],
+    "kv_cache_write": ["warp_row", "vector_rows"],
+    "kv_cache_read": ["warp_row", "vector_rows"],
+    "paged_attention": ["cta_head", "split_keys"],
+}
 
-# arguments an op takes between its tensors and the variant
-EXTRA_ARGS: dict[str, tuple] = {"layernorm": (LAYERNORM_EPS,)}
+ALL_STAGES: dict[str, list[str]] = {**CUDA_STAGES, **DECODE_STAGES}
+
+BEST_VARIANT: dict[str, int] = {k: len(v) - 1 for k, v in ALL_STAGES.items()}
+
+# arguments an op takes between its tensors and the variant: eps; eps and whether adjacent
+# elements pair up; the dtype e4m3 rows are read in; the score scale (1/sqrt(D))
+EXTRA_ARGS: dict[str, tuple] = {
+    "layernorm": (LAYERNORM_EPS,),
+    "qk_norm_rope": (NORM_EPS, False),
+    "qk_norm_rope_backward": (NORM_EPS, False),
+    "kv_cache_read": (torch.bfloat16,),
+    "paged_attention": (None,),
+}
 
 
 def _cuda_impl(kernel: str, variant: int) -> Callable:
     extra = EXTRA_ARGS.get(kernel, ())
 
     def run(*inputs):
-        return getattr(ext.ops(), kernel)(*inputs, *extra, variant)
+        args = extra
+        if kernel == "kv_cache_read" and inputs[0].dtype != torch.float8_e4m3fn:
+            args = (inputs[0].dtype,)  # plain caches are read in their own dtype
+        return getattr(ext.ops(), kernel)(*inputs, *args, variant)
 
-    run.__name__ = f"cuda_{kernel}_{CUDA_STAGES[kernel][variant]}"
+    run.__name__ = f"cuda_{kernel}_{ALL_STAGES[kernel][variant]}"
     return run
 
 
@@ -48,7 +74,7 @@ def cuda_impls(kernel: str) -> dict[str, Callable]:
     if not ext.load():
         return {}
     return {f"cuda:{stage}": _cuda_impl(kernel, i)
-            for i, stage in enumerate(CUDA_STAGES.get(kernel, []))}
+            for i, stage in enumerate(ALL_STAGES.get(kernel, []))}
 
 
 def best(kernel: str) -> Callable:
@@ -59,7 +85,7 @@ def best(kernel: str) -> Callable:
 
 def get_impls(kernel: str, include: tuple[str, ...] = ("torch", "cuda")
               ) -> dict[str, Callable]:
-    spec = get_spec(kernel)
+    spec = DECODE_SPECS[kernel] if kernel in DECODE_SPECS else get_spec(kernel)
     impls: dict[str, Callable] = {}
     if "torch" in include:
         impls["torch"] = spec.baseline
