@@ -340,8 +340,9 @@ def test_slots_outside_the_cache(D, variant):
 def attention_limit(q, kc, vc, table, lens, ks, vs, scale=None):
     """fp32 part of the output, per head: a score is a sum of D products, each off by up to
     2^-23 of their magnitudes' sum per addition; a weight carries that twice (its own and the
-    sum's), and 2^-16 where the weights enter the products as two 16-bit parts; the sum over
-    keys adds at most n / 4 + 32 roundings in a row."""
+    sum's), and 2^-15 where the weights enter the products as two 16-bit parts (bf16 cut
+    towards zero leaves up to 2^-7 of the weight, and that is rounded to 2^-8 of itself); the
+    sum over keys adds at most n / 4 + 32 roundings in a row."""
     B, Hq, D = q.shape
     Hkv, page = kc.shape[1:3]
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -357,7 +358,7 @@ def attention_limit(q, kc, vc, table, lens, ks, vs, scale=None):
         a = (qq.abs() @ k.abs().transpose(1, 2)).amax(-1) * scale
         w = torch.softmax(qq @ k.transpose(1, 2) * scale, dim=-1)
         av = (w @ v.abs()).amax(-1)
-        out[b, :, 0] = ((4 * (D + 16) * U23 * a + 2.0 ** -16 + (n / 4 + 32) * U23)
+        out[b, :, 0] = ((4 * (D + 16) * U23 * a + 2.0 ** -15 + (n / 4 + 32) * U23)
                         * av).reshape(Hq)
     return out
 
