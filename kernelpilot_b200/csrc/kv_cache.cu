@@ -6,6 +6,11 @@
 // read: the same rows back out by slot, codes times scale; slots below zero give zeros.
 //
 //   variant 0  one warp per (token, head), lanes strided over the row's elements
+//   variant 1  a row's 16-byte vectors (of the uncompressed side) over neighbouring lanes,
+//              key and value row of a (token, head) loaded together before either is used;
+//              one short-lived thread per vector pair, so the scheduler keeps every SM's
+//              loads in flight. Needs rows of whole vectors on vector boundaries; other
+//              layouts take variant 0.
 #include "kp_kv_cache.cuh"
 
 namespace kpb {
@@ -89,12 +94,204 @@ read_warp_row(const C* __restrict__ k_cache, const C* __restrict__ v_cache,
   }
 }
 
+// ------------------------------------------------------------------ variant 1
+
+constexpr int kVecThreads = 256;
+
+// N codes of a vector, packed.
+template <int N>
+struct Codes {
+  using type = std::conditional_t<N == 8, uint2, uint32_t>;
+};
+
+template <typename T>
+__device__ __forceinline__ typename Codes<Vec<T>::kN>::type pack_codes(const float* f, float inv) {
+  constexpr int N = Vec<T>::kN;
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    float g[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = inv == 0.f ? 0.f : f[4 * i + j] * inv;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE, __NV_E4M3);
+    w[i] = lo | hi << 16;
+  }
+  if constexpr (N == 8) return make_uint2(w[0], w[1]);
+  else return w[0];
+}
+
+template <int N>
+__device__ __forceinline__ void unpack_codes(const typename Codes<N>::type& v, float scale,
+                                             float* f) {
+  uint32_t w[2];
+  if constexpr (N == 8) { w[0] = v.x; w[1] = v.y; } else { w[0] = v; }
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const auto two = static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i % 2 * 16));
+    const float2 p = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    f[2 * i] = p.x * scale;
+    f[2 * i + 1] = p.y * scale;
+  }
+}
+
+// 2^log_lanes lanes per row, V vectors each (lane, lane + lanes): lanes * V >= row vectors.
+template <typename T, typename C, int V>
+__global__ void __launch_bounds__(kVecThreads)
+write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
+                  const int64_t* __restrict__ slots, C* k_cache, C* v_cache, float* k_scale,
+                  float* v_scale, int rows, int log_lanes, int64_t k_stride, int64_t v_stride,
+                  KvLayout lay, unsigned* err) {
+  constexpr int N = Vec<T>::kN;
+  const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * kVecThreads + threadIdx.x) >> log_lanes;
+  const bool live = group < rows;  // a group past the last row still joins the shuffles
+  const int row = static_cast<int>(group);
+  const int heads = static_cast<int>(lay.heads), nv = static_cast<int>(lay.dim) / N;
+  const int t = live ? row / heads : 0, h = live ? row - t * heads : 0;
+  const uint64_t pol = evict_first_policy();
+  const uint4* src[2] = {reinterpret_cast<const uint4*>(k + t * k_stride + h * lay.dim),
+                         reinterpret_cast<const uint4*>(v + t * v_stride + h * lay.dim)};
+  uint4 raw[2][V];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = lane + i * lanes;
+      raw[w][i] = live && j < nv ? ld_stream(src[w] + j, pol) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  int64_t page = 0, off = 0;
+  const bool store = live && locate(lay, slots[t], &page, &off, err) == 0;
+  const int64_t at = lay.row(page, h, off);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    C* y = (w == 0 ? k_cache : v_cache) + at;
+    if constexpr (std::is_same_v<C, uint8_t>) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float f[N];
+        unpack<T>(raw[w][i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) amax = max(amax, __float_as_uint(f[e]) & 0x7fffffffu);
+      }
+      for (int o = lanes >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(kFull, amax, o));
+      float inv;
+      const float s = e4m3_row_scale(amax, &inv);
+      if (!store) continue;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int j = lane + i * lanes;
+        float f[N];
+        unpack<T>(raw[w][i], f);
+        if (j < nv) reinterpret_cast<typename Codes<N>::type*>(y)[j] = pack_codes<T>(f, inv);
+      }
+      if (lane == 0) (w == 0 ? k_scale : v_scale)[lay.scale(page, h, off)] = s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int j = lane + i * lanes;
+        if (store && j < nv) reinterpret_cast<uint4*>(y)[j] = raw[w][i];
+      }
+    }
+  }
+}
+
+template <typename T, typename C, int V>
+__global__ void __launch_bounds__(kVecThreads)
+read_vector_rows(const C* __restrict__ k_cache, const C* __restrict__ v_cache,
+                 const int64_t* __restrict__ slots, const float* __restrict__ k_scale,
+                 const float* __restrict__ v_scale, T* __restrict__ k, T* __restrict__ v,
+                 int rows, int log_lanes, KvLayout lay, unsigned* err) {
+  constexpr int N = Vec<T>::kN;
+  using Held = std::conditional_t<std::is_same_v<C, uint8_t>, typename Codes<N>::type, uint4>;
+  const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kVecThreads + threadIdx.x) >> log_lanes;
+  if (row >= rows) return;
+  const int heads = static_cast<int>(lay.heads), nv = static_cast<int>(lay.dim) / N;
+  const int t = static_cast<int>(row) / heads, h = static_cast<int>(row) - t * heads;
+  int64_t page = 0, off = 0;
+  const int state = locate(lay, slots[t], &page, &off, err);
+  const int64_t at = lay.row(page, h, off);
+  Held raw[2][V] = {};
+  float scale[2] = {1.f, 1.f};
+  if (state == 0) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const Held* src = reinterpret_cast<const Held*>((w == 0 ? k_cache : v_cache) + at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int j = lane + i * lanes;
+        if (j < nv) raw[w][i] = __ldg(src + j);
+      }
+    }
+    if constexpr (std::is_same_v<C, uint8_t>) {
+      scale[0] = k_scale[lay.scale(page, h, off)];
+      scale[1] = v_scale[lay.scale(page, h, off)];
+    }
+  }
+  const float fill = state == 1 ? 0.f : nan_f();  // padding, or a slot out of range
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    uint4* y = reinterpret_cast<uint4*>((w == 0 ? k : v) + row * lay.dim);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = lane + i * lanes;
+      if (j >= nv) continue;
+      if constexpr (std::is_same_v<C, T>) {
+        if (state == 0) {
+          st_stream(y + j, raw[w][i]);
+          continue;
+        }
+      }
+      float f[N];
+      if constexpr (std::is_same_v<C, uint8_t>) unpack_codes<N>(raw[w][i], scale[w], f);
+      if (state != 0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = fill;
+      }
+      st_stream(y + j, pack<T>(f));
+    }
+  }
+}
+
 // ------------------------------------------------------------------ launch
 
+uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Rows of the cache in whole vectors of N elements on their boundaries, N being 16 bytes of
+// T; the scratch of lanes per row and vectors per lane.
 template <typename T, typename C>
-int launch_write(const void* k, const void* v, const int64_t* slots, void* k_cache,
+bool vector_rows(const KvLayout& lay, const void* k_cache, const void* v_cache) {
+  constexpr int N = Vec<T>::kN;
+  return lay.dim % N == 0 && (addr(k_cache) | addr(v_cache)) % (N * sizeof(C)) == 0 &&
+         (lay.num_pages < 2 || lay.page_stride % N == 0);
+}
+
+int lanes_log2(int64_t vectors) {
+  int log = 0;
+  while ((1 << log) < vectors && log < 5) ++log;
+  return log;
+}
+
+template <typename T, typename C>
+int launch_write(int variant, const void* k, const void* v, const int64_t* slots, void* k_cache,
                  void* v_cache, float* k_scale, float* v_scale, int64_t tokens, int64_t k_stride,
                  int64_t v_stride, const KvLayout& lay, unsigned* err, cudaStream_t s) {
+  constexpr int N = Vec<T>::kN;
+  if (variant == 1 && vector_rows<T, C>(lay, k_cache, v_cache) &&
+      (addr(k) | addr(v)) % 16 == 0 && (tokens < 2 || (k_stride | v_stride) % N == 0)) {
+    const int64_t nv = lay.dim / N;
+    const int log = lanes_log2(nv), rows = static_cast<int>(tokens * lay.heads);
+    const auto ctas = static_cast<unsigned>(cdiv(static_cast<int64_t>(rows) << log, kVecThreads));
+    auto* kernel = nv <= 32 ? write_vector_rows<T, C, 1> : write_vector_rows<T, C, 2>;
+    kernel<<<ctas, kVecThreads, 0, s>>>(
+        static_cast<const T*>(k), static_cast<const T*>(v), slots, static_cast<C*>(k_cache),
+        static_cast<C*>(v_cache), k_scale, v_scale, rows, log, k_stride, v_stride, lay, err);
+    KPB_LAUNCHED("kv_cache_write vector rows");
+    return KPB_OK;
+  }
   const auto ctas = static_cast<unsigned>(cdiv(tokens * lay.heads, kWarpsPerCta));
   write_warp_row<T, C><<<ctas, kWarpsPerCta * kWarp, 0, s>>>(
       static_cast<const T*>(k), static_cast<const T*>(v), slots, static_cast<C*>(k_cache),
@@ -104,9 +301,21 @@ int launch_write(const void* k, const void* v, const int64_t* slots, void* k_cac
 }
 
 template <typename T, typename C>
-int launch_read(const void* k_cache, const void* v_cache, const int64_t* slots,
+int launch_read(int variant, const void* k_cache, const void* v_cache, const int64_t* slots,
                 const float* k_scale, const float* v_scale, void* k, void* v, int64_t tokens,
                 const KvLayout& lay, unsigned* err, cudaStream_t s) {
+  constexpr int N = Vec<T>::kN;
+  if (variant == 1 && vector_rows<T, C>(lay, k_cache, v_cache) && (addr(k) | addr(v)) % 16 == 0) {
+    const int64_t nv = lay.dim / N;
+    const int log = lanes_log2(nv), rows = static_cast<int>(tokens * lay.heads);
+    const auto ctas = static_cast<unsigned>(cdiv(static_cast<int64_t>(rows) << log, kVecThreads));
+    auto* kernel = nv <= 32 ? read_vector_rows<T, C, 1> : read_vector_rows<T, C, 2>;
+    kernel<<<ctas, kVecThreads, 0, s>>>(
+        static_cast<const C*>(k_cache), static_cast<const C*>(v_cache), slots, k_scale, v_scale,
+        static_cast<T*>(k), static_cast<T*>(v), rows, log, lay, err);
+    KPB_LAUNCHED("kv_cache_read vector rows");
+    return KPB_OK;
+  }
   const auto ctas = static_cast<unsigned>(cdiv(tokens * lay.heads, kWarpsPerCta));
   read_warp_row<T, C><<<ctas, kWarpsPerCta * kWarp, 0, s>>>(
       static_cast<const C*>(k_cache), static_cast<const C*>(v_cache), slots, k_scale, v_scale,
@@ -122,7 +331,7 @@ int kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, const
                    float* v_scale, int64_t tokens, int64_t k_stride, int64_t v_stride,
                    const KvLayout& lay, unsigned* err, cudaStream_t s) {
 #define KPB_WRITE(T, C)                                                                      \
-  launch_write<T, C>(k, v, slots, k_cache, v_cache, k_scale, v_scale, tokens, k_stride,      \
+  launch_write<T, C>(variant, k, v, slots, k_cache, v_cache, k_scale, v_scale, tokens, k_stride,      \
                      v_stride, lay, err, s)
   const bool q = cache_dtype == KPB_E4M3;
   switch (dtype) {
@@ -138,7 +347,7 @@ int kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cache,
                   const float* v_scale, void* k, void* v, int64_t tokens, const KvLayout& lay,
                   unsigned* err, cudaStream_t s) {
 #define KPB_READ(T, C) \
-  launch_read<T, C>(k_cache, v_cache, slots, k_scale, v_scale, k, v, tokens, lay, err, s)
+  launch_read<T, C>(variant, k_cache, v_cache, slots, k_scale, v_scale, k, v, tokens, lay, err, s)
   const bool q = cache_dtype == KPB_E4M3;
   switch (dtype) {
     case KPB_F32: return q ? KPB_READ(float, uint8_t) : KPB_READ(float, float);

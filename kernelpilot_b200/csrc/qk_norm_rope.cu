@@ -14,9 +14,18 @@
 // table gives NaN rows and sets kErrIndex.
 //
 //   variant 0  one warp per row, lanes strided over its elements
+//   variant 1  a lane holds two vectors of a row that rotate with one another (i and
+//              i + rot/2), so no value crosses lanes but the row's sums; rows of D = 128
+//              16-bit values take 8 lanes. A lane keeps its angles (and weights) for
+//              several heads of the token. The backward is one wave of CTAs, some for q
+//              and some for k, each lane adding its elements' weight gradients in
+//              registers over all its rows. Needs both parts of the row (rotated and not)
+//              in whole pairs of vectors on vector boundaries (16 bytes, or 8 for 16-bit
+//              types); other layouts take variant 0.
 #include <algorithm>
 
 #include "kp_kv_cache.cuh"
+#include "kp_sm100.cuh"
 
 namespace kpb {
 namespace {
@@ -162,39 +171,440 @@ rope_back_warp_row(const T* __restrict__ gq, const T* __restrict__ gk, const T* 
   }
 }
 
-// dw[which][i] = sum over CTAs of partials[cta][which][i], in CTA order within each of the
-// block's 8 rows of threads and then in row order: the same bits every time.
+// ------------------------------------------------------------------ variant 1
+
+constexpr int kVecThreads = 256;
+
+template <int Bytes>
+struct Raw {
+  using type = std::conditional_t<Bytes == 16, uint4, uint2>;
+};
+
+template <typename T, int VE>
+using RawOf = typename Raw<VE * static_cast<int>(sizeof(T))>::type;
+
+// Streamed load of one vector: not kept in L1, first to leave L2.
+template <typename R>
+__device__ __forceinline__ R load_stream(const void* p, uint64_t pol) {
+  if constexpr (sizeof(R) == 16) {
+    return ld_stream(p, pol);
+  } else {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v2.u32 {%0,%1}, [%2], %3;"
+                 : "=r"(v.x), "=r"(v.y) : "l"(p), "l"(pol));
+    return v;
+  }
+}
+
+template <typename T, int VE, typename R>
+__device__ __forceinline__ void unpack_raw(const R& v, float* f) {
+  if constexpr (sizeof(R) == 16) {
+    unpack<T>(v, f);
+  } else {
+    float g[8];
+    unpack<T>(make_uint4(v.x, v.y, 0u, 0u), g);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = g[e];
+  }
+}
+
+template <typename T, int VE>
+__device__ __forceinline__ void store_raw(T* p, const float* f) {
+  if constexpr (VE * sizeof(T) == 16) {
+    st_stream(p, pack<T>(f));
+  } else {
+    float g[8] = {};
+#pragma unroll
+    for (int e = 0; e < VE; ++e) g[e] = f[e];
+    const uint4 v = pack<T>(g);
+    *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y);
+  }
+}
+
+// Where pair `p` of a row lies: vectors at a and b, turned by the angles from `angle` on
+// (vector a) and `angle2` on (vector b; adjacent pairs only).
+struct PairPlace {
+  int a, b, angle, angle2;
+  bool turned;
+};
+
+template <int VE>
+__device__ __forceinline__ PairPlace pair_place(int p, const RopeShape& sh) {
+  const int rot = static_cast<int>(sh.rot), dim = static_cast<int>(sh.dim);
+  PairPlace w;
+  w.turned = p * 2 * VE < rot;
+  const int from = w.turned ? 0 : rot, half = (w.turned ? rot : dim - rot) / 2;
+  w.a = from + (p * VE - (w.turned ? 0 : rot / 2));
+  w.b = w.a + half;
+  w.angle = sh.interleaved ? w.a / 2 : w.a;
+  w.angle2 = w.b / 2;
+  return w;
+}
+
+// cos and sin of the lane's angles: of elements e of both vectors (pairs rot/2 apart), or of
+// pairs e of vector a (first half) and of vector b (second half of the array).
+template <int VE>
+__device__ __forceinline__ void load_angles(const float* __restrict__ row, const PairPlace& w,
+                                            const RopeShape& sh, bool ok, float* c, float* s) {
+  const int half = static_cast<int>(sh.rot) / 2;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    c[e] = 1.f;
+    s[e] = 0.f;
+  }
+  if (!w.turned || !ok) return;
+  if (!sh.interleaved) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(row + w.angle + e));
+      const float4 y = __ldg(reinterpret_cast<const float4*>(row + half + w.angle + e));
+      c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
+      s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE / 2; ++e) {
+      c[e] = __ldg(row + w.angle + e);
+      s[e] = __ldg(row + half + w.angle + e);
+      c[VE / 2 + e] = __ldg(row + w.angle2 + e);
+      s[VE / 2 + e] = __ldg(row + half + w.angle2 + e);
+    }
+  }
+}
+
+// Turns vectors x and y of a pair; `sign` -1 turns back.
+template <int VE>
+__device__ __forceinline__ void turn(float* x, float* y, const float* c, const float* s,
+                                     float sign, bool interleaved) {
+  if (!interleaved) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float a = x[e], b = y[e], d = s[e] * sign;
+      x[e] = fmaf(a, c[e], -b * d);
+      y[e] = fmaf(b, c[e], a * d);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE / 2; ++e) {
+      float a = x[2 * e], b = x[2 * e + 1], d = s[e] * sign;
+      x[2 * e] = fmaf(a, c[e], -b * d);
+      x[2 * e + 1] = fmaf(b, c[e], a * d);
+      a = y[2 * e], b = y[2 * e + 1], d = s[VE / 2 + e] * sign;
+      y[2 * e] = fmaf(a, c[VE / 2 + e], -b * d);
+      y[2 * e + 1] = fmaf(b, c[VE / 2 + e], a * d);
+    }
+  }
+}
+
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+// A group of 2^log_lanes lanes takes HPG heads (all of q or all of k) of one token.
+template <typename T, int VE, int HPG>
+__global__ void __launch_bounds__(kVecThreads)
+rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ wq,
+                  const T* __restrict__ wk, const float* __restrict__ cos_sin,
+                  const int64_t* __restrict__ positions, T* __restrict__ q_out,
+                  T* __restrict__ k_out, int64_t q_stride, int64_t k_stride, int log_lanes,
+                  RopeShape sh, unsigned* err) {
+  using R = RawOf<T, VE>;
+  const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+  const int hq = static_cast<int>(sh.q_heads), hk = static_cast<int>(sh.k_heads);
+  const int dim = static_cast<int>(sh.dim);
+  const int q_parts = (hq + HPG - 1) / HPG, parts = q_parts + (hk + HPG - 1) / HPG;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kVecThreads + threadIdx.x) >> log_lanes;
+  const bool live = item < sh.tokens * parts;  // the rest still join the shuffles
+  const int t = live ? static_cast<int>(static_cast<uint32_t>(item) / parts) : 0;
+  const int part = live ? static_cast<int>(item) - t * parts : 0;
+  const bool is_q = part < q_parts;
+  const int h0 = (is_q ? part : part - q_parts) * HPG;
+  const int heads = is_q ? hq : hk;
+  const int mine = live && lane * 2 * VE < dim ? min(HPG, heads - h0) : 0;
+  const PairPlace pl = pair_place<VE>(lane, sh);
+  const T* x = (is_q ? q + t * q_stride : k + t * k_stride) + static_cast<int64_t>(h0) * dim;
+  const uint64_t pol = evict_first_policy();
+  R raw[HPG][2];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    raw[i][0] = raw[i][1] = R{};
+    if (i < mine) {
+      raw[i][0] = load_stream<R>(x + i * dim + pl.a, pol);
+      raw[i][1] = load_stream<R>(x + i * dim + pl.b, pol);
+    }
+  }
+  int64_t pos = live ? positions[t] : 0;
+  const bool bad = live && (pos < 0 || pos >= sh.max_pos);
+  if (bad) {
+    if (lane == 0) atomicOr(err, kErrIndex);
+    pos = 0;
+  }
+  float c[VE], s[VE], wa[VE], wb[VE];
+  load_angles<VE>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, c, s);
+  R ra = {}, rb = {};
+  if (mine > 0) {
+    const T* w = is_q ? wq : wk;
+    ra = __ldg(reinterpret_cast<const R*>(w + pl.a));
+    rb = __ldg(reinterpret_cast<const R*>(w + pl.b));
+  }
+  unpack_raw<T, VE>(ra, wa);
+  unpack_raw<T, VE>(rb, wb);
+  T* y = (is_q ? q_out : k_out) + (static_cast<int64_t>(t) * heads + h0) * dim;
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    float a[VE], b[VE], sq = 0.f;
+    unpack_raw<T, VE>(raw[i][0], a);
+    unpack_raw<T, VE>(raw[i][1], b);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) sq = fmaf(a[e], a[e], fmaf(b[e], b[e], sq));
+    float r = rsqrtf(group_sum(sq, lanes) / static_cast<float>(dim) + sh.eps);
+    if (bad) r = nan_f();
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      a[e] *= r * wa[e];
+      b[e] *= r * wb[e];
+    }
+    if (pl.turned) turn<VE>(a, b, c, s, 1.f, sh.interleaved);
+    if (i < mine) {
+      store_raw<T, VE>(y + i * dim + pl.a, a);
+      store_raw<T, VE>(y + i * dim + pl.b, b);
+    }
+  }
+}
+
+// CTAs [0, q_ctas) go over q's rows, the others over k's. Partial weight gradients to
+// partials[cta][dim]: lanes that hold the same elements are added within a warp by
+// halving, then the warps in order.
+template <typename T, int VE, int HPG>
+__global__ void __launch_bounds__(kVecThreads)
+rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
+                       const T* __restrict__ q, const T* __restrict__ k,
+                       const T* __restrict__ wq, const T* __restrict__ wk,
+                       const float* __restrict__ cos_sin, const int64_t* __restrict__ positions,
+                       T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ partials,
+                       int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
+                       int q_ctas, int log_lanes, RopeShape sh, unsigned* err) {
+  using R = RawOf<T, VE>;
+  __shared__ float sums[kVecThreads / kWarp][kMaxHeadDim];
+  pdl_launch_dependents();
+  const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
+  const int dim = static_cast<int>(sh.dim);
+  const bool is_q = static_cast<int>(blockIdx.x) < q_ctas;
+  const int heads = static_cast<int>(is_q ? sh.q_heads : sh.k_heads);
+  const int parts = (heads + HPG - 1) / HPG;
+  const int cta = is_q ? blockIdx.x : blockIdx.x - q_ctas;
+  const int ctas = is_q ? q_ctas : gridDim.x - q_ctas;
+  const T* x0 = is_q ? q : k;
+  const T* g0 = is_q ? gq : gk;
+  T* dx0 = is_q ? dq : dk;
+  const int64_t x_stride = is_q ? q_stride : k_stride, g_stride = is_q ? gq_stride : gk_stride;
+  const PairPlace pl = pair_place<VE>(lane, sh);
+  const bool holds = lane * 2 * VE < dim;
+  const uint64_t pol = evict_first_policy();
+  const float inv_d = 1.f / static_cast<float>(dim);
+
+  float wa[VE], wb[VE], acc_a[VE] = {}, acc_b[VE] = {};
+  R ra = {}, rb = {};
+  if (holds) {
+    const T* w = is_q ? wq : wk;
+    ra = __ldg(reinterpret_cast<const R*>(w + pl.a));
+    rb = __ldg(reinterpret_cast<const R*>(w + pl.b));
+  }
+  unpack_raw<T, VE>(ra, wa);
+  unpack_raw<T, VE>(rb, wb);
+
+  const int per_cta = kVecThreads >> log_lanes;
+  const int64_t items = sh.tokens * parts;
+  // every lane of the CTA takes the same number of turns: the shuffles need whole warps
+  for (int64_t base = static_cast<int64_t>(cta) * per_cta; base < items;
+       base += static_cast<int64_t>(ctas) * per_cta) {
+    const int64_t item = base + (threadIdx.x >> log_lanes);
+    const bool live = item < items;
+    const int t = live ? static_cast<int>(static_cast<uint32_t>(item) / parts) : 0;
+    const int h0 = live ? (static_cast<int>(item) - t * parts) * HPG : 0;
+    const int mine = live && holds ? min(HPG, heads - h0) : 0;
+    const T* x = x0 + t * x_stride + static_cast<int64_t>(h0) * dim;
+    const T* g = g0 + t * g_stride + static_cast<int64_t>(h0) * dim;
+    R rx[HPG][2], rg[HPG][2];
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      rx[i][0] = rx[i][1] = rg[i][0] = rg[i][1] = R{};
+      if (i < mine) {
+        rg[i][0] = load_stream<R>(g + i * dim + pl.a, pol);
+        rg[i][1] = load_stream<R>(g + i * dim + pl.b, pol);
+        rx[i][0] = load_stream<R>(x + i * dim + pl.a, pol);
+        rx[i][1] = load_stream<R>(x + i * dim + pl.b, pol);
+      }
+    }
+    int64_t pos = live ? positions[t] : 0;
+    const bool bad = live && (pos < 0 || pos >= sh.max_pos);
+    if (bad) {
+      if (lane == 0) atomicOr(err, kErrIndex);
+      pos = 0;
+    }
+    float c[VE], s[VE];
+    load_angles<VE>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, c, s);
+    T* dx = dx0 + (static_cast<int64_t>(t) * heads + h0) * dim;
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      float xa[VE], xb[VE], ya[VE], yb[VE], sq = 0.f, inner = 0.f;
+      unpack_raw<T, VE>(rx[i][0], xa);
+      unpack_raw<T, VE>(rx[i][1], xb);
+      unpack_raw<T, VE>(rg[i][0], ya);
+      unpack_raw<T, VE>(rg[i][1], yb);
+      if (pl.turned) turn<VE>(ya, yb, c, s, -1.f, sh.interleaved);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        sq = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], sq));
+        inner = fmaf(ya[e] * wa[e], xa[e], fmaf(yb[e] * wb[e], xb[e], inner));
+      }
+      float r = rsqrtf(group_sum(sq, lanes) * inv_d + sh.eps);
+      if (bad) r = nan_f();
+      const float m = group_sum(inner, lanes) * inv_d * r;  // mean(dn * x r)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        xa[e] *= r;
+        xb[e] *= r;
+        if (i < mine) {
+          acc_a[e] = fmaf(ya[e], xa[e], acc_a[e]);
+          acc_b[e] = fmaf(yb[e], xb[e], acc_b[e]);
+        }
+        xa[e] = r * fmaf(-xa[e], m, ya[e] * wa[e]);
+        xb[e] = r * fmaf(-xb[e], m, yb[e] * wb[e]);
+      }
+      if (i < mine) {
+        store_raw<T, VE>(dx + i * dim + pl.a, xa);
+        store_raw<T, VE>(dx + i * dim + pl.b, xb);
+      }
+    }
+  }
+  const int warp = threadIdx.x / kWarp;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    for (int o = lanes; o < kWarp; o <<= 1) {
+      acc_a[e] += __shfl_xor_sync(kFull, acc_a[e], o);
+      acc_b[e] += __shfl_xor_sync(kFull, acc_b[e], o);
+    }
+    if ((threadIdx.x & (kWarp - 1)) < lanes && holds) {
+      sums[warp][pl.a + e] = acc_a[e];
+      sums[warp][pl.b + e] = acc_b[e];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < dim; i += kVecThreads) {
+    float total = 0.f;
+#pragma unroll
+    for (int j = 0; j < kVecThreads / kWarp; ++j) total += sums[j][i];
+    partials[static_cast<int64_t>(blockIdx.x) * dim + i] = total;
+  }
+}
+
+// ------------------------------------------------------------------ weight gradients
+
+// Partials of one weight: `count` rows of dim floats, `stride` apart.
+struct Partials {
+  const float* at;
+  int64_t count, stride;
+};
+
+// dw[i] = sum of the partials: every 32nd one by one row of threads, then the 32 rows in
+// order, so the same bits every time.
+constexpr int kFinishRows = 32;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-rope_weight_finish(const float* __restrict__ partials, int64_t ctas, int dim, T* dwq, T* dwk) {
-  __shared__ float part[8][33];
-  const int which = blockIdx.y;
+__global__ void __launch_bounds__(kWarp * kFinishRows)
+rope_weight_finish(Partials pq, Partials pk, int dim, T* dwq, T* dwk) {
+  __shared__ float part[kFinishRows][kWarp + 1];
+  const Partials p = blockIdx.y == 0 ? pq : pk;
   const int lane = threadIdx.x & (kWarp - 1), slice = threadIdx.x / kWarp;
   const int i = blockIdx.x * kWarp + lane;
+  pdl_wait_primary();
   float s = 0.f;
-  if (i < dim)
-    for (int64_t c = slice; c < ctas; c += 8) s += partials[(c * 2 + which) * dim + i];
+  if (i < dim) {
+#pragma unroll 4
+    for (int64_t c = slice; c < p.count; c += kFinishRows) s += p.at[c * p.stride + i];
+  }
   part[slice][lane] = s;
   __syncthreads();
   if (slice == 0 && i < dim) {
     s = 0.f;
-    for (int j = 0; j < 8; ++j) s += part[j][lane];
-    (which == 0 ? dwq : dwk)[i] = from_f<T>(s);
+    for (int j = 0; j < kFinishRows; ++j) s += part[j][lane];
+    (blockIdx.y == 0 ? dwq : dwk)[i] = from_f<T>(s);
   }
 }
 
 // ------------------------------------------------------------------ launch
 
-// CTAs of the backward's first kernel (each writes one partial of both weights).
+// CTAs of the backward's first kernel per weight (each writes one partial).
 int64_t back_ctas(const RopeShape& sh, int sms) {
   const int64_t rows = sh.tokens * std::max(sh.q_heads, sh.k_heads);
   return std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, kWarpsPerCta), int64_t{4} * sms));
 }
 
+uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Elements of the vectors that variant 1 takes this call in, 0 where it does not: 16 bytes,
+// or 8 for 16-bit types (a rotated part of 40 elements, say, is no whole number of pairs of
+// 16-byte vectors). `all` holds the or of all addresses, `strides` of all token strides.
 template <typename T>
-int launch(const T* q, const T* k, const T* wq, const T* wk, const float* cos_sin,
+int vector_elements(const RopeShape& sh, uintptr_t all, int64_t strides, const float* cos_sin) {
+  if (addr(cos_sin) % 16 != 0) return 0;
+  for (int ve = Vec<T>::kN; ve >= 4; ve /= 2) {
+    if (sh.rot % (2 * ve) == 0 && (sh.dim - sh.rot) % (2 * ve) == 0 &&
+        all % (ve * sizeof(T)) == 0 && (sh.tokens < 2 || strides % ve == 0))
+      return ve;
+  }
+  return 0;
+}
+
+int lanes_log2(int64_t pairs) {
+  int log = 0;
+  while ((int64_t{1} << log) < pairs) ++log;
+  return log;
+}
+
+template <typename T, int VE, int HPG>
+int launch_pairs(const T* q, const T* k, const T* wq, const T* wk, const float* cos_sin,
+                 const int64_t* positions, T* q_out, T* k_out, int64_t q_stride,
+                 int64_t k_stride, const RopeShape& sh, unsigned* err, cudaStream_t s) {
+  const int log = lanes_log2(sh.dim / (2 * VE));
+  const int64_t items = sh.tokens * (cdiv(sh.q_heads, HPG) + cdiv(sh.k_heads, HPG));
+  rope_vector_pairs<T, VE, HPG>
+      <<<static_cast<unsigned>(cdiv(items << log, kVecThreads)), kVecThreads, 0, s>>>(
+          q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride, k_stride, log, sh, err);
+  KPB_LAUNCHED("qk_norm_rope vector pairs");
+  return KPB_OK;
+}
+
+// Four heads to a group once that still gives every SM 1024 threads; one where rows are few.
+template <typename T, int VE>
+int dispatch_pairs(const T* q, const T* k, const T* wq, const T* wk, const float* cos_sin,
+                   const int64_t* positions, T* q_out, T* k_out, int64_t q_stride,
+                   int64_t k_stride, const RopeShape& sh, unsigned* err, cudaStream_t s) {
+  const int64_t threads = sh.tokens * (sh.q_heads + sh.k_heads) << lanes_log2(sh.dim / (2 * VE));
+  if (threads >= int64_t{4} * 1024 * sm_count())
+    return launch_pairs<T, VE, 4>(q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride,
+                                  k_stride, sh, err, s);
+  return launch_pairs<T, VE, 1>(q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride,
+                                k_stride, sh, err, s);
+}
+
+template <typename T>
+int launch(int variant, const T* q, const T* k, const T* wq, const T* wk, const float* cos_sin,
            const int64_t* positions, T* q_out, T* k_out, int64_t q_stride, int64_t k_stride,
            const RopeShape& sh, unsigned* err, cudaStream_t s) {
+  if (variant == 1) {
+    const int ve = vector_elements<T>(
+        sh, addr(q) | addr(k) | addr(wq) | addr(wk) | addr(q_out) | addr(k_out),
+        q_stride | k_stride, cos_sin);
+    if (ve == Vec<T>::kN)
+      return dispatch_pairs<T, Vec<T>::kN>(q, k, wq, wk, cos_sin, positions, q_out, k_out,
+                                           q_stride, k_stride, sh, err, s);
+    if (ve == 4)
+      return dispatch_pairs<T, 4>(q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride,
+                                  k_stride, sh, err, s);
+  }
   const int64_t rows = sh.tokens * (sh.q_heads + sh.k_heads);
   rope_warp_row<T><<<static_cast<unsigned>(cdiv(rows, kWarpsPerCta)), kWarpsPerCta * kWarp, 0, s>>>(
       q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride, k_stride, sh, err);
@@ -203,19 +613,78 @@ int launch(const T* q, const T* k, const T* wq, const T* wk, const float* cos_si
 }
 
 template <typename T>
-int launch_back(const T* gq, const T* gk, const T* q, const T* k, const T* wq, const T* wk,
-                const float* cos_sin, const int64_t* positions, T* dq, T* dk, T* dwq, T* dwk,
-                int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
+int finish_weights(const Partials& pq, const Partials& pk, int dim, T* dwq, T* dwk, bool dependent,
+                   cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(cdiv(dim, kWarp)), 2);
+  cfg.blockDim = dim3(kWarp * kFinishRows);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  KPB_CUDA(cudaLaunchKernelEx(&cfg, rope_weight_finish<T>, pq, pk, dim, dwq, dwk));
+  return KPB_OK;
+}
+
+template <typename T, int VE>
+int launch_back_pairs(const T* gq, const T* gk, const T* q, const T* k, const T* wq, const T* wk,
+                      const float* cos_sin, const int64_t* positions, T* dq, T* dk, T* dwq,
+                      T* dwk, int64_t gq_stride, int64_t gk_stride, int64_t q_stride,
+                      int64_t k_stride, const RopeShape& sh, float* partials, unsigned* err,
+                      cudaStream_t s) {
+  constexpr int HPG = 2;
+  const int dim = static_cast<int>(sh.dim), log = lanes_log2(dim / (2 * VE));
+  auto* kernel = rope_back_vector_pairs<T, VE, HPG>;
+  int occ = 0;
+  if (int rc = occupancy_blocks(reinterpret_cast<const void*>(kernel), kVecThreads, 0, &occ))
+    return rc;
+  // one wave, shared out by the heads; no more CTAs than there is work for, nor than partials
+  const int64_t wave = int64_t{occ} * sm_count(), most = back_ctas(sh, sm_count());
+  const int64_t heads = sh.q_heads + sh.k_heads;
+  const auto ctas_of = [&](int64_t h) {
+    if (h == 0 || sh.tokens == 0) return int64_t{0};
+    const int64_t items = sh.tokens * cdiv(h, HPG);
+    return std::max<int64_t>(
+        1, std::min({cdiv(items << log, kVecThreads), wave * h / heads, most}));
+  };
+  const int64_t nq = ctas_of(sh.q_heads), nk = ctas_of(sh.k_heads);
+  if (nq + nk > 0) {
+    kernel<<<static_cast<unsigned>(nq + nk), kVecThreads, 0, s>>>(
+        gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, partials, gq_stride, gk_stride,
+        q_stride, k_stride, static_cast<int>(nq), log, sh, err);
+    KPB_LAUNCHED("qk_norm_rope_backward vector pairs");
+  }
+  return finish_weights<T>({partials, nq, dim}, {partials + nq * dim, nk, dim}, dim, dwq, dwk,
+                           nq + nk > 0, s);
+}
+
+template <typename T>
+int launch_back(int variant, const T* gq, const T* gk, const T* q, const T* k, const T* wq,
+                const T* wk, const float* cos_sin, const int64_t* positions, T* dq, T* dk, T* dwq,
+                T* dwk, int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
                 const RopeShape& sh, float* partials, unsigned* err, cudaStream_t s) {
+  if (variant == 1) {
+    const int ve = vector_elements<T>(
+        sh, addr(gq) | addr(gk) | addr(q) | addr(k) | addr(wq) | addr(wk) | addr(dq) | addr(dk),
+        gq_stride | gk_stride | q_stride | k_stride, cos_sin);
+    if (ve == Vec<T>::kN)
+      return launch_back_pairs<T, Vec<T>::kN>(gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk,
+                                              dwq, dwk, gq_stride, gk_stride, q_stride, k_stride,
+                                              sh, partials, err, s);
+    if (ve == 4)
+      return launch_back_pairs<T, 4>(gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, dwq, dwk,
+                                     gq_stride, gk_stride, q_stride, k_stride, sh, partials, err,
+                                     s);
+  }
   const int64_t ctas = back_ctas(sh, sm_count());
   rope_back_warp_row<T><<<static_cast<unsigned>(ctas), kWarpsPerCta * kWarp, 0, s>>>(
       gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, partials, gq_stride, gk_stride, q_stride,
       k_stride, sh, err);
   KPB_LAUNCHED("qk_norm_rope_backward");
-  const dim3 grid(static_cast<unsigned>(cdiv(sh.dim, kWarp)), 2);
-  rope_weight_finish<T><<<grid, 256, 0, s>>>(partials, ctas, static_cast<int>(sh.dim), dwq, dwk);
-  KPB_LAUNCHED("qk_norm_rope_backward finish");
-  return KPB_OK;
+  return finish_weights<T>({partials, ctas, 2 * sh.dim}, {partials + sh.dim, ctas, 2 * sh.dim},
+                           static_cast<int>(sh.dim), dwq, dwk, false, s);
 }
 
 }  // namespace
@@ -238,7 +707,7 @@ int qk_norm_rope(int variant, int dtype, const void* q, const void* k, const voi
                  bool interleaved, unsigned* err, cudaStream_t s) {
   const RopeShape sh{tokens, q_heads, k_heads, dim, rot, max_pos, eps, interleaved};
 #define KPB_ROPE(T)                                                                       \
-  launch<T>(static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(wq), \
+  launch<T>(variant, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(wq), \
             static_cast<const T*>(wk), cos_sin, positions, static_cast<T*>(q_out),        \
             static_cast<T*>(k_out), q_stride, k_stride, sh, err, s)
   switch (dtype) {
@@ -258,7 +727,8 @@ int qk_norm_rope_backward(int variant, int dtype, const void* gq, const void* gk
                           void* ws, unsigned* err, cudaStream_t s) {
   const RopeShape sh{tokens, q_heads, k_heads, dim, rot, max_pos, eps, interleaved};
 #define KPB_ROPE(T)                                                                            \
-  launch_back<T>(static_cast<const T*>(gq), static_cast<const T*>(gk), static_cast<const T*>(q), \
+  launch_back<T>(variant, static_cast<const T*>(gq), static_cast<const T*>(gk),                \
+                 static_cast<const T*>(q),                                                     \
                  static_cast<const T*>(k), static_cast<const T*>(wq), static_cast<const T*>(wk), \
                  cos_sin, positions, static_cast<T*>(dq), static_cast<T*>(dk),                 \
                  static_cast<T*>(dwq), static_cast<T*>(dwk), gq_stride, gk_stride, q_stride,   \
