@@ -19,11 +19,12 @@ namespace {
 constexpr int kWarpsPerCta = 8;
 
 // (page, offset) of a slot. 0: in range, 1: padding (below zero), 2: out of range
-// (recorded in *err).
-__device__ __forceinline__ int locate(const KvLayout& lay, int64_t slot, int64_t* page,
-                                      int64_t* off, unsigned* err) {
+// (recorded in *err). page_log: log2 of the page size, -1 where it is no power of two (a
+// 64-bit division costs a fifth of the row's instructions).
+__device__ __forceinline__ int locate(const KvLayout& lay, int page_log, int64_t slot,
+                                      int64_t* page, int64_t* off, unsigned* err) {
   if (slot < 0) return 1;
-  *page = slot / lay.page_size;
+  *page = page_log >= 0 ? slot >> page_log : slot / lay.page_size;
   *off = slot - *page * lay.page_size;
   if (*page >= lay.num_pages) {
     atomicOr(err, kErrIndex);
@@ -45,7 +46,7 @@ write_warp_row(const T* __restrict__ k, const T* __restrict__ v,
   if (row >= tokens * lay.heads) return;
   const int64_t t = row / lay.heads, h = row - t * lay.heads;
   int64_t page, off;
-  if (locate(lay, slots[t], &page, &off, err) != 0) return;
+  if (locate(lay, -1, slots[t], &page, &off, err) != 0) return;
   const int64_t at = lay.row(page, h, off), sat = lay.scale(page, h, off);
   for (int which = 0; which < 2; ++which) {
     const T* x = which == 0 ? k + t * k_stride + h * lay.dim : v + t * v_stride + h * lay.dim;
@@ -76,7 +77,7 @@ read_warp_row(const C* __restrict__ k_cache, const C* __restrict__ v_cache,
   if (row >= tokens * lay.heads) return;
   const int64_t t = row / lay.heads, h = row - t * lay.heads;
   int64_t page = 0, off = 0;
-  const int state = locate(lay, slots[t], &page, &off, err);
+  const int state = locate(lay, -1, slots[t], &page, &off, err);
   const int64_t at = lay.row(page, h, off), sat = lay.scale(page, h, off);
   for (int which = 0; which < 2; ++which) {
     T* y = (which == 0 ? k : v) + row * lay.dim;
@@ -104,6 +105,30 @@ struct Codes {
   using type = std::conditional_t<N == 8, uint2, uint32_t>;
 };
 
+// The largest magnitude's bits of a vector: over packed pairs for the 16-bit types, whose
+// patterns order as their fp32 values do (infinities and NaNs above the rest).
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+  } else {
+    return __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  }
+}
+
+// The pattern of max_bits over a row as that of an fp32 value.
+template <typename T>
+__device__ __forceinline__ uint32_t as_f32_bits(uint32_t v) {
+  if constexpr (sizeof(T) == 4) {
+    return v;
+  } else {
+    const uint32_t top = max(v & 0xffffu, v >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) return top << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top))));
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ typename Codes<Vec<T>::kN>::type pack_codes(const float* f, float inv) {
   constexpr int N = Vec<T>::kN;
@@ -112,7 +137,7 @@ __device__ __forceinline__ typename Codes<Vec<T>::kN>::type pack_codes(const flo
   for (int i = 0; i < N / 4; ++i) {
     float g[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = inv == 0.f ? 0.f : f[4 * i + j] * inv;
+    for (int j = 0; j < 4; ++j) g[j] = f[4 * i + j] * inv;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE, __NV_E4M3);
     w[i] = lo | hi << 16;
@@ -140,7 +165,7 @@ template <typename T, typename C, int V>
 __global__ void __launch_bounds__(kVecThreads)
 write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
                   const int64_t* __restrict__ slots, C* k_cache, C* v_cache, float* k_scale,
-                  float* v_scale, int rows, int log_lanes, int64_t k_stride, int64_t v_stride,
+                  float* v_scale, int rows, int log_lanes, int page_log, int64_t k_stride, int64_t v_stride,
                   KvLayout lay, unsigned* err) {
   constexpr int N = Vec<T>::kN;
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
@@ -162,7 +187,7 @@ write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
     }
   }
   int64_t page = 0, off = 0;
-  const bool store = live && locate(lay, slots[t], &page, &off, err) == 0;
+  const bool store = live && locate(lay, page_log, slots[t], &page, &off, err) == 0;
   const int64_t at = lay.row(page, h, off);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
@@ -171,21 +196,24 @@ write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
       uint32_t amax = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float f[N];
-        unpack<T>(raw[w][i], f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) amax = max(amax, __float_as_uint(f[e]) & 0x7fffffffu);
+        const uint32_t top = max_bits<T>(raw[w][i]);
+        amax = sizeof(T) == 4 ? max(amax, top) : __vmaxu2(amax, top);
       }
-      for (int o = lanes >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(kFull, amax, o));
+      for (int o = lanes >> 1; o > 0; o >>= 1) {
+        const uint32_t other = __shfl_xor_sync(kFull, amax, o);
+        amax = sizeof(T) == 4 ? max(amax, other) : __vmaxu2(amax, other);
+      }
       float inv;
-      const float s = e4m3_row_scale(amax, &inv);
+      const float s = e4m3_row_scale(as_f32_bits<T>(amax), &inv);
       if (!store) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int j = lane + i * lanes;
         float f[N];
         unpack<T>(raw[w][i], f);
-        if (j < nv) reinterpret_cast<typename Codes<N>::type*>(y)[j] = pack_codes<T>(f, inv);
+        typename Codes<N>::type codes = pack_codes<T>(f, inv);
+        if (inv == 0.f) codes = typename Codes<N>::type{};  // a row that is not finite: NaN * 0 is no code of 0
+        if (j < nv) reinterpret_cast<typename Codes<N>::type*>(y)[j] = codes;
       }
       if (lane == 0) (w == 0 ? k_scale : v_scale)[lay.scale(page, h, off)] = s;
     } else {
@@ -203,7 +231,7 @@ __global__ void __launch_bounds__(kVecThreads)
 read_vector_rows(const C* __restrict__ k_cache, const C* __restrict__ v_cache,
                  const int64_t* __restrict__ slots, const float* __restrict__ k_scale,
                  const float* __restrict__ v_scale, T* __restrict__ k, T* __restrict__ v,
-                 int rows, int log_lanes, KvLayout lay, unsigned* err) {
+                 int rows, int log_lanes, int page_log, KvLayout lay, unsigned* err) {
   constexpr int N = Vec<T>::kN;
   using Held = std::conditional_t<std::is_same_v<C, uint8_t>, typename Codes<N>::type, uint4>;
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
@@ -212,7 +240,7 @@ read_vector_rows(const C* __restrict__ k_cache, const C* __restrict__ v_cache,
   const int heads = static_cast<int>(lay.heads), nv = static_cast<int>(lay.dim) / N;
   const int t = static_cast<int>(row) / heads, h = static_cast<int>(row) - t * heads;
   int64_t page = 0, off = 0;
-  const int state = locate(lay, slots[t], &page, &off, err);
+  const int state = locate(lay, page_log, slots[t], &page, &off, err);
   const int64_t at = lay.row(page, h, off);
   Held raw[2][V] = {};
   float scale[2] = {1.f, 1.f};
@@ -269,9 +297,20 @@ bool vector_rows(const KvLayout& lay, const void* k_cache, const void* v_cache) 
          (lay.num_pages < 2 || lay.page_stride % N == 0);
 }
 
+// Two vectors of each row to a lane, so that a row's fixed work (its slot, its scale) falls
+// on half the threads; 32 lanes then hold the longest row (fp32, D = 256).
+constexpr int kPerRowLane = 2;
+
 int lanes_log2(int64_t vectors) {
   int log = 0;
-  while ((1 << log) < vectors && log < 5) ++log;
+  while ((kPerRowLane << log) < vectors) ++log;
+  return log;
+}
+
+int log2_of(int64_t n) {  // -1 where n is no power of two
+  if ((n & (n - 1)) != 0) return -1;
+  int log = 0;
+  while (int64_t{1} << log < n) ++log;
   return log;
 }
 
@@ -285,10 +324,10 @@ int launch_write(int variant, const void* k, const void* v, const int64_t* slots
     const int64_t nv = lay.dim / N;
     const int log = lanes_log2(nv), rows = static_cast<int>(tokens * lay.heads);
     const auto ctas = static_cast<unsigned>(cdiv(static_cast<int64_t>(rows) << log, kVecThreads));
-    auto* kernel = nv <= 32 ? write_vector_rows<T, C, 1> : write_vector_rows<T, C, 2>;
-    kernel<<<ctas, kVecThreads, 0, s>>>(
+    write_vector_rows<T, C, kPerRowLane><<<ctas, kVecThreads, 0, s>>>(
         static_cast<const T*>(k), static_cast<const T*>(v), slots, static_cast<C*>(k_cache),
-        static_cast<C*>(v_cache), k_scale, v_scale, rows, log, k_stride, v_stride, lay, err);
+        static_cast<C*>(v_cache), k_scale, v_scale, rows, log, log2_of(lay.page_size), k_stride,
+        v_stride, lay, err);
     KPB_LAUNCHED("kv_cache_write vector rows");
     return KPB_OK;
   }
@@ -309,10 +348,10 @@ int launch_read(int variant, const void* k_cache, const void* v_cache, const int
     const int64_t nv = lay.dim / N;
     const int log = lanes_log2(nv), rows = static_cast<int>(tokens * lay.heads);
     const auto ctas = static_cast<unsigned>(cdiv(static_cast<int64_t>(rows) << log, kVecThreads));
-    auto* kernel = nv <= 32 ? read_vector_rows<T, C, 1> : read_vector_rows<T, C, 2>;
-    kernel<<<ctas, kVecThreads, 0, s>>>(
+    read_vector_rows<T, C, kPerRowLane><<<ctas, kVecThreads, 0, s>>>(
         static_cast<const C*>(k_cache), static_cast<const C*>(v_cache), slots, k_scale, v_scale,
-        static_cast<T*>(k), static_cast<T*>(v), rows, log, lay, err);
+        static_cast<T*>(k), static_cast<T*>(v), rows, log, log2_of(lay.page_size), lay,
+        err);
     KPB_LAUNCHED("kv_cache_read vector rows");
     return KPB_OK;
   }

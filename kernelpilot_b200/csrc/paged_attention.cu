@@ -132,10 +132,8 @@ paged_cta_head(const T* __restrict__ q, const C* __restrict__ k_cache,
 
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * kWarp;
-constexpr int kWarpKeys = 16;
-constexpr int kUnit = kSplitWarps * kWarpKeys;  // keys of a row per unit of work
 
-// How rows and units are laid out: rows of a sequence are (key head, tile of `tile_heads`
+// How rows and units are laid out: a unit is `unit` keys of a row; rows of a sequence are (key head, tile of `tile_heads`
 // query heads), tiles innermost; a partial has tile_heads x (pitch) floats: pitch - 4
 // weighted values, then maximum and sum.
 struct SplitShape {
@@ -144,9 +142,15 @@ struct SplitShape {
   int group;         // query heads per key head
   int tile_heads;
   int pitch;
+  int unit_log;      // log2 of the keys per unit
   int64_t* bases;    // workspace: units before each sequence (batch), then their total
   float* partials;   // workspace: [cta][2][tile_heads][pitch]
 };
+
+// Units of a row of n keys.
+__device__ __forceinline__ int units_of(int64_t n, const SplitShape& sp) {
+  return static_cast<int>((n + (1 << sp.unit_log) - 1) >> sp.unit_log);
+}
 
 __device__ __forceinline__ int64_t first_unit(int64_t cta, int64_t ctas, int64_t total) {
   return cta * total / ctas;
@@ -157,22 +161,22 @@ __device__ __forceinline__ int64_t cta_of_unit(int64_t u, int64_t ctas, int64_t 
   return ((u + 1) * ctas - 1) / total;
 }
 
-// A place in the list of units: sequence, row, block of kUnit keys.
+// A place in the list of units: sequence, row, block of keys.
 struct UnitPlace {
   int64_t b, row;
   int blk, blocks;  // block within the row, blocks of the row
   int n;            // keys of the sequence
 
   __device__ __forceinline__ void next(const int* __restrict__ seq_lens, const PagedShape& sh,
-                                       int64_t rows, unsigned* err) {
+                                       const SplitShape& sp, unsigned* err) {
     if (++blk < blocks) return;
     blk = 0;
-    if (++row < rows) return;
+    if (++row < sp.rows) return;
     row = 0;
     do {
       ++b;
       n = b < sh.batch ? static_cast<int>(keys_of(seq_lens, b, sh, err)) : 1;
-      blocks = (n + kUnit - 1) / kUnit;
+      blocks = units_of(n, sp);
     } while (blocks == 0);
   }
 };
@@ -188,7 +192,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   const int64_t b0 = min(sh.batch, threadIdx.x * per), b1 = min(sh.batch, b0 + per);
   int64_t mine = 0;
   for (int64_t b = b0; b < b1; ++b)
-    mine += (keys_of(seq_lens, b, sh, err) + kUnit - 1) / kUnit * sp.rows;
+    mine += units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < kWarp; o <<= 1) {
@@ -211,7 +215,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   const bool here = *begin < *end && *begin >= base && *begin < upto;
   if (blockIdx.x == 0 || here) {
     for (int64_t b = b0; b < b1; ++b) {
-      const int64_t units = (keys_of(seq_lens, b, sh, err) + kUnit - 1) / kUnit * sp.rows;
+      const int64_t units = units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
       if (blockIdx.x == 0) sp.bases[b] = base;
       if (here && *begin >= base && *begin < base + units) {
         scratch[kSplitWarps] = b;
@@ -227,7 +231,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
     p.b = scratch[kSplitWarps];
     const int64_t in = *begin - scratch[kSplitWarps + 1];
     p.n = static_cast<int>(keys_of(seq_lens, p.b, sh, err));
-    p.blocks = (p.n + kUnit - 1) / kUnit;
+    p.blocks = units_of(p.n, sp);
     p.row = in / p.blocks;
     p.blk = static_cast<int>(in - p.row * p.blocks);
   }
@@ -246,19 +250,21 @@ __device__ __forceinline__ void zero_empty(T* __restrict__ o, const int* __restr
   }
 }
 
-// Joins the warps' (maximum s_m, sum s_l, weighted values s_o; [warp][head], values
-// [warp][head][pitch]) of the segment that ends here and writes it: the output where the
-// segment is a whole row, else partial `slot` of this CTA.
+// Joins the warps' parts of the segment that ends here (maximum s_m and sum s_l,
+// [warp][head]; weighted values s_o, [warp][head - h0][pitch], of heads h0 to h0 + held of
+// the tile) and writes it: the output where the segment is a whole row, else partial `slot`
+// of this CTA.
 template <typename T>
 __device__ __forceinline__ void write_segment(const float* s_m, const float* s_l,
-                                              const float* s_o, const UnitPlace& p, bool whole,
-                                              int slot, T* __restrict__ o, const PagedShape& sh,
+                                              const float* s_o, int h0, int held,
+                                              const UnitPlace& p, bool whole, int slot,
+                                              T* __restrict__ o, const PagedShape& sh,
                                               const SplitShape& sp) {
   const int64_t hk = p.row / sp.tiles;
   const int first = static_cast<int>(p.row - hk * sp.tiles) * sp.tile_heads;
-  const int heads = min(sp.tile_heads, sp.group - first);
+  const int h1 = min(h0 + held, sp.group - first);
   const int dim = static_cast<int>(sh.lay.dim);
-  for (int h = 0; h < heads; ++h) {
+  for (int h = h0; h < h1; ++h) {
     float f[kSplitWarps], top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, s_m[w * sp.tile_heads + h]);
@@ -274,7 +280,7 @@ __device__ __forceinline__ void write_segment(const float* s_m, const float* s_l
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < kSplitWarps; ++w)
-        v = fmaf(f[w], s_o[(w * sp.tile_heads + h) * sp.pitch + i], v);
+        v = fmaf(f[w], s_o[(w * held + h - h0) * sp.pitch + i], v);
       if (whole) {
         o[(p.b * sh.q_heads + hk * sp.group + first + h) * dim + i] = from_f<T>(v / sum);
       } else {
@@ -299,13 +305,12 @@ join_rows(const int* __restrict__ seq_lens, T* __restrict__ o, PagedShape sh, Sp
           int64_t ctas, unsigned* err) {
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
   const int64_t b = blockIdx.x / sp.rows, row = blockIdx.x - b * sp.rows;
+  const int64_t blocks = units_of(keys_of(seq_lens, b, sh, err), sp);
   pdl_wait_primary();
-  const int64_t n = keys_of(seq_lens, b, sh, err);
-  const int64_t blocks = (n + kUnit - 1) / kUnit;
+  const int64_t total = sp.bases[sh.batch], base = sp.bases[b];
   if (blocks < 2) return;
-  const int64_t total = sp.bases[sh.batch];
   ctas = min(ctas, total);
-  const int64_t u0 = sp.bases[b] + row * blocks;
+  const int64_t u0 = base + row * blocks;
   const int64_t c0 = cta_of_unit(u0, ctas, total), c1 = cta_of_unit(u0 + blocks - 1, ctas, total);
   if (c0 == c1) return;
   const int64_t hk = row / sp.tiles;
@@ -364,6 +369,8 @@ __device__ __forceinline__ int64_t key_row(const int* __restrict__ table, int64_
 
 // ------------------------------------------------------------------ variant 1: split_simt
 
+constexpr int kSimtUnit = 64;
+
 // Lanes are strided over a row's elements (E each); a warp takes 4 keys at a time and HG
 // query heads: 4 * HG products, summed over the lanes by halving, so that each lane ends
 // with the score of one (key, head).
@@ -373,7 +380,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
            const int* __restrict__ table, const int* __restrict__ seq_lens,
            const float* __restrict__ k_scale, const float* __restrict__ v_scale,
            T* __restrict__ o, PagedShape sh, SplitShape sp, unsigned* err) {
-  constexpr int kKeys = 4;
+  constexpr int kKeys = 4, kWarpKeys = kSimtUnit / kSplitWarps;
   constexpr int kSums = kKeys * HG;
   constexpr int kLog = kSums == 32 ? 5 : kSums == 16 ? 4 : kSums == 8 ? 3 : 2;
   constexpr int kSpread = 5 - kLog;  // 2^kSpread neighbouring lanes hold the same sum
@@ -411,7 +418,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       l = 0.f;
       fresh = false;
     }
-    const int key0 = p.blk * kUnit + warp * kWarpKeys;
+    const int key0 = p.blk * kSimtUnit + warp * kWarpKeys;
     int64_t my_scale = 0;
     const int64_t my_row = lane < kWarpKeys
                                ? key_row(table, p.b, key0 + lane, p.n, hk, sh, &my_scale, err)
@@ -516,33 +523,17 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
           s_o[(warp * HG + hh) * kPitch + lane + e * kWarp] = acc[hh][e];
       }
       __syncthreads();
-      write_segment(s_m, s_l, s_o, p, whole_start && row_ends, slot, o, sh, sp);
+      write_segment(s_m, s_l, s_o, 0, HG, p, whole_start && row_ends, slot, o, sh, sp);
       __syncthreads();
       fresh = true;
       whole_start = true;
       slot = 1;
     }
-    p.next(seq_lens, sh, sp.rows, err);
+    p.next(seq_lens, sh, sp, err);
   }
 }
 
 // ------------------------------------------------------------------ variant 1: split_mma
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-               :: "r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-               :: "r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
-}
 
 // Four 8 x 8 blocks of 16-bit units; lane l gives the address of row l % 8 of block l / 8.
 template <bool kTrans>
@@ -610,15 +601,11 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
 // fraction down to 2^-28 of the largest weight and something down to 2^-38.
 constexpr float kWeightBits = 14.f;
 
-// Four e4m3 codes as two pairs of fp16 holding code / 256: the code's exponent and fraction
-// moved under fp16's, 8 below its bias, subnormals included. `even` takes bytes 0 and 2,
-// `odd` bytes 1 and 3.
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* even, uint32_t* odd) {
-  const uint32_t lo = w << 8;
-  *even = ((lo >> 1) & 0x3f803f80u) | (lo & 0x80008000u);
-  *odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+// Two e4m3 codes (the low 16 bits) as a pair of fp16, exactly.
+__device__ __forceinline__ uint32_t codes_to_half(uint32_t w) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
 }
-constexpr float kCodeUnit = 256.f;
 
 // Byte offset of 16-byte chunk `ch` of row `row` in a tile of rows of kRow bytes, chunks
 // exchanged so that eight rows' equal chunks lie in different banks.
@@ -632,21 +619,32 @@ __device__ __forceinline__ uint32_t tile_at(int row, int ch) {
 }
 
 // Shared memory of one CTA: kStages x (keys, values, scales) per warp, then the warps'
-// meeting place. kStages fills half an SM (two CTAs), 2 at least and 4 at most.
+// meeting place, kMeetHeads heads at a time. A warp takes 32 keys at a time where a row is
+// 128 bytes at most, else 16. As many stages as let three CTAs share an SM, two at least
+// and four at most; with two that do not fit, two CTAs or one.
+constexpr int kMeetHeads = 4;
+
 template <typename C, int DP, int NT>
 struct MmaPlan {
   static constexpr bool kQuant = std::is_same_v<C, uint8_t>;
   static constexpr int kRow = DP * static_cast<int>(sizeof(C));
-  static constexpr int kTile = kWarpKeys * kRow;
-  static constexpr int kStage = 2 * kTile + (kQuant ? 2 * kWarpKeys * 4 : 0);
+  static constexpr int kKeys = kRow <= 128 && DP * NT <= 128 ? 32 : 16;
+  static constexpr int kUnit = kSplitWarps * kKeys;
+  static constexpr int kTile = kKeys * kRow;
+  static constexpr int kStage = 2 * kTile + (kQuant ? 2 * kKeys * 4 : 0);
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPitch = DP + 4;
-  static constexpr int kMeet = kSplitWarps * kHeads * (kPitch + 2) * 4 + 64;
-  static constexpr int kHalfSm = 228 * 1024 / 2 - 1024;
-  static constexpr int kFit = (kHalfSm - kMeet) / (kSplitWarps * kStage);
+  static constexpr int kMeet = kSplitWarps * (2 * kHeads + kMeetHeads * kPitch) * 4 + 64;
+  static constexpr int kThirdSm = 228 * 1024 / 3 - 1024;
+  static constexpr int kFit = (kThirdSm - kMeet) / (kSplitWarps * kStage);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
   static constexpr int kSmem = kSplitWarps * kStages * kStage + kMeet;
 };
+
+// Rows of the cache as the loader holds them: 16-byte units from the cache's start, in 32
+// bits (mma_takes bounds the cache), or one of two marks.
+constexpr uint32_t kNoRow = 0xffffffffu;   // past the last key
+constexpr uint32_t kBadRow = 0xfffffffeu;  // in a page outside the cache
 
 // T: q and o. C: the cache (T, or e4m3 codes). DP: head dim, padded with zeros. NT: tiles
 // of 8 query heads.
@@ -669,13 +667,14 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   using M = std::conditional_t<Plan::kQuant, __half, T>;  // operand type of the products
   constexpr bool kQuant = Plan::kQuant;
   constexpr int kS = Plan::kStages, kRow = Plan::kRow, kHeads = Plan::kHeads;
+  constexpr int kKeys = Plan::kKeys, kTiles = kKeys / 16;
   constexpr int kChunks = kRow / 16;
   constexpr int kSteps = DP / 16;
   extern __shared__ __align__(128) unsigned char smem[];
   float* s_m = reinterpret_cast<float*>(smem + kSplitWarps * kS * Plan::kStage);
   float* s_l = s_m + kSplitWarps * kHeads;
   float* s_o = s_l + kSplitWarps * kHeads;
-  auto* scratch = reinterpret_cast<int64_t*>(s_o + kSplitWarps * kHeads * Plan::kPitch);
+  auto* scratch = reinterpret_cast<int64_t*>(s_o + kSplitWarps * kMeetHeads * Plan::kPitch);
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
   const int r = lane >> 2, t = lane & 3;  // row and column pair of this lane's fragments
   const int dim = static_cast<int>(sh.lay.dim);
@@ -689,38 +688,54 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   if (u >= end) return;
 
   // The loader runs kS - 1 units ahead, and looks up its next unit's pages one unit before
-  // that: next_row / next_scale are those of this lane's key (lane % 16).
+  // that: next_row / next_scale are those of this lane's key (lane % kKeys).
   UnitPlace lp = p;
-  int64_t lu = u, next_row = -1, next_scale = 0;
+  int left = static_cast<int>(end - u);  // units that the loader has not begun
+  uint32_t next_row = kNoRow, next_scale = 0;
   unsigned bad_slots = 0;
+  const auto page_size = static_cast<uint32_t>(sh.lay.page_size);
+  const auto page_units = static_cast<uint32_t>(sh.lay.page_stride * sizeof(C) / 16);
   auto look_up = [&]() {
-    next_row = -1;
-    if (lu < end)
-      next_row = key_row(table, lp.b, lp.blk * kUnit + warp * kWarpKeys + (lane & 15), lp.n,
-                         lp.row / sp.tiles, sh, &next_scale, err);
+    next_row = kNoRow;
+    const uint32_t pos = lp.blk * Plan::kUnit + warp * kKeys + (lane & (kKeys - 1));
+    if (left <= 0 || pos >= static_cast<uint32_t>(lp.n)) return;
+    const uint32_t at = pos / page_size, off = pos - at * page_size;
+    const int page = table[lp.b * sh.table_stride + at];
+    if (page < 0 || page >= sh.lay.num_pages) {
+      atomicOr(err, kErrIndex);
+      next_row = kBadRow;
+      return;
+    }
+    const uint32_t hk = static_cast<uint32_t>(lp.row) / sp.tiles;
+    next_row = page * page_units + (hk * page_size + off) * chunks_in;
+    next_scale = (page * static_cast<uint32_t>(sh.lay.heads) + hk) * page_size + off;
   };
   auto load = [&](int stage) {
-    if (lu < end) {
+    if (left > 0) {
       const uint32_t kd = ring + stage * Plan::kStage, vd = kd + Plan::kTile;
-      const bool bad = __any_sync(kFull, next_row == -2);
+      const bool bad = __any_sync(kFull, next_row == kBadRow);
       bad_slots = bad ? bad_slots | (1u << stage) : bad_slots & ~(1u << stage);
 #pragma unroll
-      for (int i = 0; i < kChunks / 2; ++i) {
+      for (int i = 0; i < kKeys * kChunks / kWarp; ++i) {
         const int c = i * kWarp + lane;
         const int row = c / kChunks, ch = c % kChunks;
-        const int64_t at = __shfl_sync(kFull, next_row, row);
-        const bool in = at >= 0 && ch < chunks_in;
-        const int64_t byte = in ? at * static_cast<int64_t>(sizeof(C)) + ch * 16 : 0;
+        const uint32_t at = __shfl_sync(kFull, next_row, row);
+        const bool in = at < kBadRow && ch < chunks_in;
+        const uint64_t byte = in ? static_cast<uint64_t>(at + ch) * 16 : 0;
         cp_async16(kd + tile_at<kRow>(row, ch), reinterpret_cast<const char*>(k_cache) + byte, in);
         cp_async16(vd + tile_at<kRow>(row, ch), reinterpret_cast<const char*>(v_cache) + byte, in);
       }
-      if constexpr (kQuant) {  // 16 key scales, then 16 value scales
-        const bool in = next_row >= 0;
-        cp_async4(vd + Plan::kTile + lane * 4, (lane < 16 ? k_scale : v_scale) + (in ? next_scale : 0),
-                  in);
+      if constexpr (kQuant) {  // the key scales, then the value scales
+        const bool in = next_row < kBadRow;
+        const uint32_t at = in ? next_scale : 0, sd = vd + Plan::kTile + lane * 4;
+        if constexpr (kKeys == 32) {
+          cp_async4(sd, k_scale + at, in);
+          cp_async4(sd + 128, v_scale + at, in);
+        } else {
+          cp_async4(sd, (lane < 16 ? k_scale : v_scale) + at, in);
+        }
       }
-      ++lu;
-      if (lu < end) lp.next(seq_lens, sh, sp.rows, err);
+      if (--left > 0) lp.next(seq_lens, sh, sp, err);
     }
     cp_async_commit();  // an empty group where nothing is left, so that the count stays
     look_up();
@@ -735,10 +750,10 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   float m[NT][2], l[NT][2], mo[NT][2];    // running maximum, sum; maximum of weight * scale
   bool fresh = true, whole_start = p.blk == 0;
   int slot = 0, stage = 0;
-  for (; u < end; ++u) {
-    const int64_t hk = p.row / sp.tiles;
+  for (int units = static_cast<int>(end - u); units > 0; --units) {
     if (fresh) {
       fresh = false;
+      const int64_t hk = p.row / sp.tiles;
       const int first = static_cast<int>(p.row - hk * sp.tiles) * kHeads;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -757,7 +772,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           }
           mult[nt][0] = mult[nt][1] = sh.scale * kLog2e;
         } else {
-          // elements 4t .. 4t+3 of each 16; even ones pair up, and odd ones, as the codes do
+          // elements 4t .. 4t+3 of each 16, in the order that a word of codes has them
           uint32_t top = 0;
 #pragma unroll
           for (int kk = 0; kk < kSteps; ++kk) {
@@ -781,17 +796,16 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           const float down = __uint_as_float((254 - ex) << 23), up = __uint_as_float(ex << 23);
 #pragma unroll
           for (int kk = 0; kk < kSteps; ++kk) {
-            const T* a = reinterpret_cast<const T*>(&qb[nt][kk][0]);
-            const T* b = reinterpret_cast<const T*>(&qb[nt][kk][1]);
-            const float x0 = to_f(a[0]) * down, x1 = to_f(a[1]) * down;
-            const float x2 = to_f(b[0]) * down, x3 = to_f(b[1]) * down;
-            const __half2 ev = __floats2half2_rn(x0, x2), od = __floats2half2_rn(x1, x3);
-            qb[nt][kk][0] = *reinterpret_cast<const uint32_t*>(&ev);
-            qb[nt][kk][1] = *reinterpret_cast<const uint32_t*>(&od);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const T* e = reinterpret_cast<const T*>(&qb[nt][kk][i]);
+              const __half2 v = __floats2half2_rn(to_f(e[0]) * down, to_f(e[1]) * down);
+              qb[nt][kk][i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
           }
           // `up` of heads 2t and 2t + 1 lies with the lanes of rows 2t and 2t + 1
-          mult[nt][0] = __shfl_sync(kFull, up, 8 * t) * (sh.scale * kLog2e * kCodeUnit);
-          mult[nt][1] = __shfl_sync(kFull, up, 8 * t + 4) * (sh.scale * kLog2e * kCodeUnit);
+          mult[nt][0] = __shfl_sync(kFull, up, 8 * t) * (sh.scale * kLog2e);
+          mult[nt][1] = __shfl_sync(kFull, up, 8 * t + 4) * (sh.scale * kLog2e);
         }
 #pragma unroll
         for (int kk = 0; kk < kSteps; ++kk) {
@@ -807,83 +821,108 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     cp_async_wait<kS - 1>();
     __syncwarp();
     const uint32_t kt = ring + stage * Plan::kStage, vt = kt + Plan::kTile;
-    const int key0 = p.blk * kUnit + warp * kWarpKeys;
+    const int key0 = p.blk * Plan::kUnit + warp * kKeys;
     if (key0 < p.n) {  // else none of this warp's keys is left in the row
       // scores: block l / 8 of an ldmatrix is keys (l / 8) % 2 * 8 .., chunk + l / 16
       const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
-      float c[NT][2][4] = {};
-      if constexpr (!kQuant) {
+      float c[kTiles][NT][2][4] = {};
 #pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          uint32_t a[4];
-          ldmatrix4<false>(kt + tile_at<kRow>(krow, 2 * kk + kch), a);
+      for (int j = 0; j < kTiles; ++j) {
+        if constexpr (!kQuant) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816<M>(c[nt][kk & 1], a[0], a[1], a[2], a[3], qb[nt][kk][0], qb[nt][kk][1]);
-        }
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < kSteps; kk += 2) {
-          uint32_t w[4];
-          ldmatrix4<false>(kt + tile_at<kRow>(krow, kk + kch), w);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half(w[2 * i], &a0, &a2);
-            codes_to_half(w[2 * i + 1], &a1, &a3);
+          for (int kk = 0; kk < kSteps; ++kk) {
+            uint32_t a[4];
+            ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, 2 * kk + kch), a);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<M>(c[nt][i], a0, a1, a2, a3, qb[nt][kk + i][0], qb[nt][kk + i][1]);
+              mma16816<M>(c[j][nt][kk & 1], a[0], a[1], a[2], a[3], qb[nt][kk][0], qb[nt][kk][1]);
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < kSteps; kk += 2) {
+            uint32_t w[4];
+            ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a0 = codes_to_half(w[2 * i]), a1 = codes_to_half(w[2 * i + 1]);
+              const uint32_t a2 = codes_to_half(w[2 * i] >> 16);
+              const uint32_t a3 = codes_to_half(w[2 * i + 1] >> 16);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<M>(c[j][nt][i], a0, a1, a2, a3, qb[nt][kk + i][0], qb[nt][kk + i][1]);
+            }
           }
         }
       }
-      float ks[2] = {1.f, 1.f}, vlog[2] = {0.f, 0.f};
+      float ks[kTiles][2], vlog[kTiles][2];
       if constexpr (kQuant) {
         const float* sc = reinterpret_cast<const float*>(
             smem + (warp * kS + stage) * Plan::kStage + 2 * Plan::kTile);
-        ks[0] = sc[r];
-        ks[1] = sc[r + 8];
-        vlog[0] = __log2f(sc[16 + r]);
-        vlog[1] = __log2f(sc[16 + r + 8]);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ks[j][h] = sc[16 * j + 8 * h + r];
+            vlog[j][h] = __log2f(sc[kKeys + 16 * j + 8 * h + r]);
+          }
+        }
       }
-      const bool in0 = key0 + r < p.n, in1 = key0 + r + 8 < p.n;
-      uint32_t hi[NT][2], lo[NT][2];
+      const bool full = key0 + kKeys <= p.n;
+      uint32_t hi[kTiles][NT][2], lo[kTiles][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float s[2][2];  // [key r, r + 8][head 2t, 2t + 1]
+        float w[kTiles][2][2], alpha[2];  // [16 keys][key r, r + 8][head 2t, 2t + 1]
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[0][i] = in0 ? (c[nt][0][i] + c[nt][1][i]) * (mult[nt][i] * ks[0]) : -INFINITY;
-          s[1][i] = in1 ? (c[nt][0][2 + i] + c[nt][1][2 + i]) * (mult[nt][i] * ks[1]) : -INFINITY;
-        }
-        float w[2][2], alpha[2];
+          float top = -INFINITY, vtop = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float top = fmaxf(s[0][i], s[1][i]);
+          for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
-          for (int off = 4; off < kWarp; off <<= 1)
+            for (int h = 0; h < 2; ++h) {
+              float s = c[j][nt][0][2 * h + i] + c[j][nt][1][2 * h + i];
+              s *= kQuant ? mult[nt][i] * ks[j][h] : mult[nt][i];
+              if (!full && key0 + 16 * j + 8 * h + r >= p.n) s = -INFINITY;
+              w[j][h][i] = s;
+              top = fmaxf(top, s);
+              // past the last key the scale's place holds 0: log2 gives -inf there
+              if constexpr (kQuant) vtop = fmaxf(vtop, s + vlog[j][h]);
+            }
+          }
+#pragma unroll
+          for (int off = 4; off < kWarp; off <<= 1) {
             top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+            if constexpr (kQuant) vtop = fmaxf(vtop, __shfl_xor_sync(kFull, vtop, off));
+          }
           const float m_new = fmaxf(m[nt][i], top);
           const float base = m_new == -INFINITY ? 0.f : m_new;
           alpha[i] = ex2f(m[nt][i] - base);
-          w[0][i] = ex2f(s[0][i] - (base - kWeightBits));
-          w[1][i] = ex2f(s[1][i] - (base - kWeightBits));
-          l[nt][i] = fmaf(l[nt][i], alpha[i], w[0][i] + w[1][i]);
-          m[nt][i] = m_new;
+          float sum = 0.f;
           if constexpr (kQuant) {
-            // past the last key the scale's place holds 0 and s is -inf: log2 gives -inf too
-            const float t0 = s[0][i] + vlog[0], t1 = s[1][i] + vlog[1];
-            float vtop = fmaxf(t0, t1);
-#pragma unroll
-            for (int off = 4; off < kWarp; off <<= 1)
-              vtop = fmaxf(vtop, __shfl_xor_sync(kFull, vtop, off));
             const float mo_new = fmaxf(mo[nt][i], vtop);
             const float vbase = mo_new == -INFINITY ? 0.f : mo_new;
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                sum += ex2f(w[j][h][i] - (base - kWeightBits));
+                w[j][h][i] = ex2f(w[j][h][i] + vlog[j][h] - (vbase - kWeightBits));
+              }
+            }
+            l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
             alpha[i] = ex2f(mo[nt][i] - vbase);
-            w[0][i] = ex2f(t0 - (vbase - kWeightBits));
-            w[1][i] = ex2f(t1 - (vbase - kWeightBits));
             mo[nt][i] = mo_new;
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
+                sum += w[j][h][i];
+              }
+            }
+            l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
           }
+          m[nt][i] = m_new;
         }
         if (__any_sync(kFull, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -892,39 +931,50 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
             for (int i = 0; i < 4; ++i) acc[nt][kk][i] *= alpha[i & 1];
           }
         }
-        hi[nt][0] = transpose8(split_weights<M>(w[0][0], w[0][1], &lo[nt][0]));
-        hi[nt][1] = transpose8(split_weights<M>(w[1][0], w[1][1], &lo[nt][1]));
-        lo[nt][0] = transpose8(lo[nt][0]);
-        lo[nt][1] = transpose8(lo[nt][1]);
-      }
-      // values, transposed on the way: 16-bit blocks are (keys 0-7, elements 0-7), (0-7,
-      // 8-15), (8-15, 0-7), (8-15, 8-15); e4m3 blocks as for the keys
-      if constexpr (!kQuant) {
-        const int vrow = (lane & 7) + (lane >> 4) * 8, vch = (lane >> 3) & 1;
 #pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          uint32_t a[4];
-          ldmatrix4<true>(vt + tile_at<kRow>(vrow, 2 * kk + vch), a);
+        for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], hi[nt][0], hi[nt][1]);
-            mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], lo[nt][0], lo[nt][1]);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t rest;
+            hi[j][nt][h] = transpose8(split_weights<M>(w[j][h][0], w[j][h][1], &rest));
+            lo[j][nt][h] = transpose8(rest);
           }
         }
-      } else {
+      }
+      // values, transposed on the way: 16-bit blocks are (keys 0-7, elements 0-7), (0-7,
+      // 8-15), (8-15, 0-7), (8-15, 8-15); e4m3 blocks as for the keys, two neighbouring
+      // elements of a key to a 16-bit unit
 #pragma unroll
-        for (int kk = 0; kk < kSteps; kk += 2) {
-          uint32_t w[4];
-          ldmatrix4<true>(vt + tile_at<kRow>(krow, kk + kch), w);
+      for (int j = 0; j < kTiles; ++j) {
+        if constexpr (!kQuant) {
+          const int vrow = (lane & 7) + (lane >> 4) * 8 + 16 * j, vch = (lane >> 3) & 1;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half(w[2 * i], &a0, &a1);
-            codes_to_half(w[2 * i + 1], &a2, &a3);
+          for (int kk = 0; kk < kSteps; ++kk) {
+            uint32_t a[4];
+            ldmatrix4<true>(vt + tile_at<kRow>(vrow, 2 * kk + vch), a);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
-              mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+              mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], hi[j][nt][0], hi[j][nt][1]);
+              mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], lo[j][nt][0], lo[j][nt][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < kSteps; kk += 2) {
+            uint32_t w[4];
+            ldmatrix4<true>(vt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              // bytes: key 2t (two elements), key 2t + 1 (two) -> element by element
+              const uint32_t x = __byte_perm(w[2 * i], 0, 0x3120);
+              const uint32_t y = __byte_perm(w[2 * i + 1], 0, 0x3120);
+              const uint32_t a0 = codes_to_half(x), a1 = codes_to_half(x >> 16);
+              const uint32_t a2 = codes_to_half(y), a3 = codes_to_half(y >> 16);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, hi[j][nt][0], hi[j][nt][1]);
+                mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, lo[j][nt][0], lo[j][nt][1]);
+              }
             }
           }
         }
@@ -938,10 +988,11 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     stage = stage + 1 == kS ? 0 : stage + 1;
 
     const bool row_ends = p.blk + 1 == p.blocks;
-    if (row_ends || u + 1 == end) {
+    if (row_ends || units == 1) {
+      const int heads = min(kHeads, sp.group - static_cast<int>(p.row % sp.tiles) * kHeads);
+      float f[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float sum = l[nt][i];
@@ -951,30 +1002,37 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
             s_m[warp * kHeads + nt * 8 + 2 * t + i] = m[nt][i];
             s_l[warp * kHeads + nt * 8 + 2 * t + i] = sum;
           }
-          // values of e4m3 rows are relative to the other maximum, in units of 1/256
-          f[i] = 1.f;
+          // values of e4m3 rows are relative to the other maximum
+          f[nt][i] = 1.f;
           if constexpr (kQuant)
-            f[i] = mo[nt][i] == -INFINITY ? 1.f : ex2f(mo[nt][i] - m[nt][i]) * kCodeUnit;
-        }
-#pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          const int d0 = kk * 16 + (kQuant ? 2 * r : r), d1 = d0 + (kQuant ? 1 : 8);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float* at = s_o + (warp * kHeads + nt * 8 + 2 * t + i) * Plan::kPitch;
-            at[d0] = acc[nt][kk][i] * f[i];
-            at[d1] = acc[nt][kk][2 + i] * f[i];
-          }
+            f[nt][i] = mo[nt][i] == -INFINITY ? 1.f : ex2f(mo[nt][i] - m[nt][i]);
         }
       }
-      __syncthreads();
-      write_segment(s_m, s_l, s_o, p, whole_start && row_ends, slot, o, sh, sp);
-      __syncthreads();
+#pragma unroll
+      for (int h0 = 0; h0 < kHeads; h0 += kMeetHeads) {
+        if (h0 >= heads) break;
+        const int nt = h0 / 8, at_t = t - (h0 % 8) / 2;  // this round's heads: nt, t of 0 .. 1
+        if (at_t == 0 || at_t == 1) {
+#pragma unroll
+          for (int kk = 0; kk < kSteps; ++kk) {
+            const int d0 = kk * 16 + (kQuant ? 2 * r : r), d1 = d0 + (kQuant ? 1 : 8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float* at = s_o + (warp * kMeetHeads + 2 * at_t + i) * Plan::kPitch;
+              at[d0] = acc[nt][kk][i] * f[nt][i];
+              at[d1] = acc[nt][kk][2 + i] * f[nt][i];
+            }
+          }
+        }
+        __syncthreads();
+        write_segment(s_m, s_l, s_o, h0, kMeetHeads, p, whole_start && row_ends, slot, o, sh, sp);
+        __syncthreads();
+      }
       fresh = true;
       whole_start = true;
       slot = 1;
     }
-    p.next(seq_lens, sh, sp.rows, err);
+    p.next(seq_lens, sh, sp, err);
   }
   cp_async_wait<0>();
 }
@@ -1003,8 +1061,8 @@ size_t bases_bytes(int64_t batch) {
 }
 
 // Units of a call if every sequence were as long as its table allows.
-int64_t units_bound(int64_t batch, int64_t rows, int64_t max_len) {
-  const int64_t per = cdiv(max_len, kUnit) * rows;
+int64_t units_bound(int64_t batch, int64_t rows, int64_t max_len, int unit) {
+  const int64_t per = cdiv(max_len, unit) * rows;
   return per == 0 ? 0 : batch > INT64_MAX / 4096 / per ? INT64_MAX / 4096 : batch * per;
 }
 
@@ -1016,7 +1074,7 @@ int64_t split_ctas(int64_t units, int64_t resident) {
 template <typename T>
 int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
   const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
-  if (max_len <= kUnit) return KPB_OK;  // no row has a second unit to share
+  if (max_len <= int64_t{1} << sp.unit_log) return KPB_OK;  // no row has a second unit to share
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c.sh.batch * sp.rows));
   cfg.blockDim = dim3(kJoinWarps * kWarp);
@@ -1031,13 +1089,15 @@ int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
   return KPB_OK;
 }
 
-SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, void* ws) {
+SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, void* ws) {
   SplitShape sp;
   sp.group = static_cast<int>(c.sh.q_heads / c.sh.lay.heads);
   sp.tile_heads = tile_heads;
   sp.tiles = static_cast<int>(cdiv(sp.group, tile_heads));
   sp.rows = c.sh.lay.heads * sp.tiles;
   sp.pitch = pitch;
+  for (sp.unit_log = 0; 1 << sp.unit_log < unit; ++sp.unit_log) {
+  }
   sp.bases = static_cast<int64_t*>(ws);
   sp.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + bases_bytes(c.sh.batch));
   return sp;
@@ -1045,12 +1105,12 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, void* ws) 
 
 template <typename T, typename C, int E, int HG>
 int launch_simt(const PagedCall& c, void* ws) {
-  const SplitShape sp = split_shape(c, HG, E * kWarp + 4, ws);
+  const SplitShape sp = split_shape(c, HG, E * kWarp + 4, kSimtUnit, ws);
   auto* kernel = split_simt<T, C, E, HG>;
   int occ = 0;
   if (int rc = occupancy_blocks(reinterpret_cast<const void*>(kernel), kSplitThreads, 0, &occ))
     return rc;
-  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size);
+  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, kSimtUnit);
   const int64_t ctas = split_ctas(units, int64_t{occ} * sm_count());
   kernel<<<static_cast<unsigned>(ctas), kSplitThreads, 0, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
@@ -1080,13 +1140,13 @@ int dispatch_simt(const PagedCall& c, void* ws) {
 template <typename T, typename C, int DP, int NT>
 int launch_mma(const PagedCall& c, void* ws) {
   using Plan = MmaPlan<C, DP, NT>;
-  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, ws);
+  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, Plan::kUnit, ws);
   auto* kernel = split_mma<T, C, DP, NT>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   if (int rc = ensure_dyn_smem(fn, Plan::kSmem)) return rc;
   int occ = 0;
   if (int rc = occupancy_blocks(fn, kSplitThreads, Plan::kSmem, &occ)) return rc;
-  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size);
+  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, Plan::kUnit);
   const int64_t ctas = split_ctas(units, int64_t{occ} * sm_count());
   kernel<<<static_cast<unsigned>(ctas), kSplitThreads, Plan::kSmem, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
@@ -1109,13 +1169,14 @@ int dispatch_mma(const PagedCall& c, void* ws) {
 }
 
 // Rows of the cache whole 16-byte chunks on 16-byte boundaries (cp.async), q's rows on
-// 8-byte ones.
+// 8-byte ones; the cache's 16-byte units counted in 32 bits (64 GB, of 180 on the card).
 template <typename C>
 bool mma_takes(const PagedCall& c) {
   const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   return c.sh.lay.dim * sizeof(C) % 16 == 0 && c.sh.lay.dim % 8 == 0 &&
          (at(c.k_cache) | at(c.v_cache)) % 16 == 0 &&
          (c.sh.lay.num_pages < 2 || c.sh.lay.page_stride * sizeof(C) % 16 == 0) &&
+         c.sh.lay.num_pages * c.sh.lay.page_stride * static_cast<int64_t>(sizeof(C)) / 16 < kBadRow &&
          at(c.q) % 8 == 0 && (c.sh.batch < 2 || c.sh.q_stride % 4 == 0);
 }
 
@@ -1144,7 +1205,7 @@ size_t paged_attention_workspace_bytes(int variant, int64_t batch, int64_t q_hea
   // there can be units (a tile holds one head at least)
   const int pitch = static_cast<int>(dim <= 64 ? 64 : dim <= 128 ? 128 : 256) + 4;
   const int heads = q_heads / k_heads > 8 && dim <= 128 ? 16 : 8;
-  const int64_t ctas = split_ctas(units_bound(batch, q_heads, max_len), kMaxCtas);
+  const int64_t ctas = split_ctas(units_bound(batch, q_heads, max_len, kSimtUnit), kMaxCtas);
   return bases_bytes(batch) +
          static_cast<size_t>(ctas * partial_floats(heads, pitch)) * sizeof(float);
 }

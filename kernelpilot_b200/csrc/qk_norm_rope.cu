@@ -173,7 +173,8 @@ rope_back_warp_row(const T* __restrict__ gq, const T* __restrict__ gk, const T* 
 
 // ------------------------------------------------------------------ variant 1
 
-constexpr int kVecThreads = 256;
+constexpr int kRopeThreads = 128;  // forward
+constexpr int kVecThreads = 256;   // backward
 
 template <int Bytes>
 struct Raw {
@@ -196,30 +197,37 @@ __device__ __forceinline__ R load_stream(const void* p, uint64_t pol) {
   }
 }
 
+// A vector's VE elements as VE / 2 packed pairs of floats, and back.
 template <typename T, int VE, typename R>
-__device__ __forceinline__ void unpack_raw(const R& v, float* f) {
+__device__ __forceinline__ void unpack_raw(const R& v, float2* f) {
+  float g[8];
   if constexpr (sizeof(R) == 16) {
-    unpack<T>(v, f);
+    unpack<T>(v, g);
   } else {
-    float g[8];
     unpack<T>(make_uint4(v.x, v.y, 0u, 0u), g);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = g[e];
   }
+#pragma unroll
+  for (int e = 0; e < VE / 2; ++e) f[e] = make_float2(g[2 * e], g[2 * e + 1]);
 }
 
 template <typename T, int VE>
-__device__ __forceinline__ void store_raw(T* p, const float* f) {
-  if constexpr (VE * sizeof(T) == 16) {
-    st_stream(p, pack<T>(f));
-  } else {
-    float g[8] = {};
+__device__ __forceinline__ void store_raw(T* p, const float2* f) {
+  float g[8] = {};
 #pragma unroll
-    for (int e = 0; e < VE; ++e) g[e] = f[e];
-    const uint4 v = pack<T>(g);
+  for (int e = 0; e < VE / 2; ++e) {
+    g[2 * e] = f[e].x;
+    g[2 * e + 1] = f[e].y;
+  }
+  const uint4 v = pack<T>(g);
+  if constexpr (VE * sizeof(T) == 16) {
+    st_stream(p, v);
+  } else {
     *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y);
   }
 }
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
 
 // Where pair `p` of a row lies: vectors at a and b, turned by the angles from `angle` on
 // (vector a) and `angle2` on (vector b; adjacent pairs only).
@@ -228,7 +236,7 @@ struct PairPlace {
   bool turned;
 };
 
-template <int VE>
+template <int VE, bool kAdjacent>
 __device__ __forceinline__ PairPlace pair_place(int p, const RopeShape& sh) {
   const int rot = static_cast<int>(sh.rot), dim = static_cast<int>(sh.dim);
   PairPlace w;
@@ -236,74 +244,69 @@ __device__ __forceinline__ PairPlace pair_place(int p, const RopeShape& sh) {
   const int from = w.turned ? 0 : rot, half = (w.turned ? rot : dim - rot) / 2;
   w.a = from + (p * VE - (w.turned ? 0 : rot / 2));
   w.b = w.a + half;
-  w.angle = sh.interleaved ? w.a / 2 : w.a;
+  w.angle = kAdjacent ? w.a / 2 : w.a;
   w.angle2 = w.b / 2;
   return w;
 }
 
-// cos and sin of the lane's angles: of elements e of both vectors (pairs rot/2 apart), or of
-// pairs e of vector a (first half) and of vector b (second half of the array).
-template <int VE>
+// Cosines and sines for the lane's two vectors, as packed pairs. Pairs rot/2 apart share
+// them: (a, b) turns to (a c - b s, b c + a s), and cb, sb are left alone. With adjacent
+// pairs a turns to a * ca + swapped(a) * sa, sa = (-sin, sin), and b likewise.
+template <int VE, bool kAdjacent>
 __device__ __forceinline__ void load_angles(const float* __restrict__ row, const PairPlace& w,
-                                            const RopeShape& sh, bool ok, float* c, float* s) {
+                                            const RopeShape& sh, bool ok, float2* ca, float2* sa,
+                                            float2* cb, float2* sb) {
   const int half = static_cast<int>(sh.rot) / 2;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    c[e] = 1.f;
-    s[e] = 0.f;
+  for (int e = 0; e < VE / 2; ++e) {
+    ca[e] = both(1.f);
+    sa[e] = both(0.f);
+    if constexpr (kAdjacent) {
+      cb[e] = both(1.f);
+      sb[e] = both(0.f);
+    }
   }
   if (!w.turned || !ok) return;
-  if (!sh.interleaved) {
+  if constexpr (!kAdjacent) {
 #pragma unroll
     for (int e = 0; e < VE; e += 4) {
       const float4 x = __ldg(reinterpret_cast<const float4*>(row + w.angle + e));
       const float4 y = __ldg(reinterpret_cast<const float4*>(row + half + w.angle + e));
-      c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
-      s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
+      ca[e / 2] = make_float2(x.x, x.y);
+      ca[e / 2 + 1] = make_float2(x.z, x.w);
+      sa[e / 2] = make_float2(y.x, y.y);
+      sa[e / 2 + 1] = make_float2(y.z, y.w);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < VE / 2; ++e) {
-      c[e] = __ldg(row + w.angle + e);
-      s[e] = __ldg(row + half + w.angle + e);
-      c[VE / 2 + e] = __ldg(row + w.angle2 + e);
-      s[VE / 2 + e] = __ldg(row + half + w.angle2 + e);
+      ca[e] = both(__ldg(row + w.angle + e));
+      cb[e] = both(__ldg(row + w.angle2 + e));
+      const float s = __ldg(row + half + w.angle + e), s2 = __ldg(row + half + w.angle2 + e);
+      sa[e] = make_float2(-s, s);
+      sb[e] = make_float2(-s2, s2);
     }
   }
 }
 
-// Turns vectors x and y of a pair; `sign` -1 turns back.
-template <int VE>
-__device__ __forceinline__ void turn(float* x, float* y, const float* c, const float* s,
-                                     float sign, bool interleaved) {
-  if (!interleaved) {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const float a = x[e], b = y[e], d = s[e] * sign;
-      x[e] = fmaf(a, c[e], -b * d);
-      y[e] = fmaf(b, c[e], a * d);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < VE / 2; ++e) {
-      float a = x[2 * e], b = x[2 * e + 1], d = s[e] * sign;
-      x[2 * e] = fmaf(a, c[e], -b * d);
-      x[2 * e + 1] = fmaf(b, c[e], a * d);
-      a = y[2 * e], b = y[2 * e + 1], d = s[VE / 2 + e] * sign;
-      y[2 * e] = fmaf(a, c[VE / 2 + e], -b * d);
-      y[2 * e + 1] = fmaf(b, c[VE / 2 + e], a * d);
-    }
-  }
-}
+__device__ __forceinline__ float2 swapped(float2 v) { return make_float2(v.y, v.x); }
 
 __device__ __forceinline__ float group_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
 
+__device__ __forceinline__ float2 group_sum2(float2 v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(kFull, v.x, o);
+    v.y += __shfl_xor_sync(kFull, v.y, o);
+  }
+  return v;
+}
+
 // A group of 2^log_lanes lanes takes HPG heads (all of q or all of k) of one token.
-template <typename T, int VE, int HPG>
-__global__ void __launch_bounds__(kVecThreads)
+template <typename T, int VE, int HPG, bool kAdjacent>
+__global__ void __launch_bounds__(kRopeThreads, 4)
 rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ wq,
                   const T* __restrict__ wk, const float* __restrict__ cos_sin,
                   const int64_t* __restrict__ positions, T* __restrict__ q_out,
@@ -314,7 +317,7 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
   const int hq = static_cast<int>(sh.q_heads), hk = static_cast<int>(sh.k_heads);
   const int dim = static_cast<int>(sh.dim);
   const int q_parts = (hq + HPG - 1) / HPG, parts = q_parts + (hk + HPG - 1) / HPG;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kVecThreads + threadIdx.x) >> log_lanes;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x) >> log_lanes;
   const bool live = item < sh.tokens * parts;  // the rest still join the shuffles
   const int t = live ? static_cast<int>(static_cast<uint32_t>(item) / parts) : 0;
   const int part = live ? static_cast<int>(item) - t * parts : 0;
@@ -322,7 +325,7 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
   const int h0 = (is_q ? part : part - q_parts) * HPG;
   const int heads = is_q ? hq : hk;
   const int mine = live && lane * 2 * VE < dim ? min(HPG, heads - h0) : 0;
-  const PairPlace pl = pair_place<VE>(lane, sh);
+  const PairPlace pl = pair_place<VE, kAdjacent>(lane, sh);
   const T* x = (is_q ? q + t * q_stride : k + t * k_stride) + static_cast<int64_t>(h0) * dim;
   const uint64_t pol = evict_first_policy();
   R raw[HPG][2];
@@ -340,8 +343,9 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
     if (lane == 0) atomicOr(err, kErrIndex);
     pos = 0;
   }
-  float c[VE], s[VE], wa[VE], wb[VE];
-  load_angles<VE>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, c, s);
+  // out_a = r (x_a pa + other(x_a) qa): the angles times the weights, once for all heads
+  float2 pa[VE / 2], qa[VE / 2], pb[VE / 2], qb[VE / 2], wa[VE / 2], wb[VE / 2];
+  load_angles<VE, kAdjacent>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, pa, qa, pb, qb);
   R ra = {}, rb = {};
   if (mine > 0) {
     const T* w = is_q ? wq : wk;
@@ -350,22 +354,38 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
   }
   unpack_raw<T, VE>(ra, wa);
   unpack_raw<T, VE>(rb, wb);
+#pragma unroll
+  for (int e = 0; e < VE / 2; ++e) {
+    if constexpr (!kAdjacent) {
+      pb[e] = pa[e];
+      qb[e] = qa[e];
+      qa[e] = neg2(qa[e]);
+    }
+    pa[e] = __fmul2_rn(pa[e], wa[e]);
+    pb[e] = __fmul2_rn(pb[e], wb[e]);
+    qa[e] = __fmul2_rn(qa[e], kAdjacent ? swapped(wa[e]) : wb[e]);
+    qb[e] = __fmul2_rn(qb[e], kAdjacent ? swapped(wb[e]) : wa[e]);
+  }
   T* y = (is_q ? q_out : k_out) + (static_cast<int64_t>(t) * heads + h0) * dim;
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
-    float a[VE], b[VE], sq = 0.f;
+    float2 a[VE / 2], b[VE / 2], sq = both(0.f);
     unpack_raw<T, VE>(raw[i][0], a);
     unpack_raw<T, VE>(raw[i][1], b);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) sq = fmaf(a[e], a[e], fmaf(b[e], b[e], sq));
-    float r = rsqrtf(group_sum(sq, lanes) / static_cast<float>(dim) + sh.eps);
+    for (int e = 0; e < VE / 2; ++e) sq = __ffma2_rn(a[e], a[e], __ffma2_rn(b[e], b[e], sq));
+    float r = rsqrtf(group_sum(sq.x + sq.y, lanes) / static_cast<float>(dim) + sh.eps);
     if (bad) r = nan_f();
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      a[e] *= r * wa[e];
-      b[e] *= r * wb[e];
+    for (int e = 0; e < VE / 2; ++e) {
+      float2 ya = __fmul2_rn(a[e], pa[e]), yb = __fmul2_rn(b[e], pb[e]);
+      if (pl.turned) {  // not 0 * other: the other may be infinite
+        ya = __ffma2_rn(kAdjacent ? swapped(a[e]) : b[e], qa[e], ya);
+        yb = __ffma2_rn(kAdjacent ? swapped(b[e]) : a[e], qb[e], yb);
+      }
+      a[e] = __fmul2_rn(ya, both(r));
+      b[e] = __fmul2_rn(yb, both(r));
     }
-    if (pl.turned) turn<VE>(a, b, c, s, 1.f, sh.interleaved);
     if (i < mine) {
       store_raw<T, VE>(y + i * dim + pl.a, a);
       store_raw<T, VE>(y + i * dim + pl.b, b);
@@ -373,11 +393,16 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
   }
 }
 
-// CTAs [0, q_ctas) go over q's rows, the others over k's. Partial weight gradients to
-// partials[cta][dim]: lanes that hold the same elements are added within a warp by
-// halving, then the warps in order.
-template <typename T, int VE, int HPG>
-__global__ void __launch_bounds__(kVecThreads)
+// CTAs [0, q_ctas) go over q's rows, the others over k's; a turn is HPG heads of a token per
+// group of lanes. A thread's own vectors come through its own slots of a shared-memory ring
+// (cp.async, kBackStages - 1 turns ahead), which takes no registers and no barrier: held in
+// registers, loads and sums together left 12 warps an SM. Partial weight gradients to
+// partials[cta][dim]: lanes that hold the same elements are added within a warp by halving,
+// then the warps in order.
+constexpr int kBackStages = 2;
+
+template <typename T, int VE, int HPG, bool kAdjacent>
+__global__ void __launch_bounds__(kVecThreads, 2)
 rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
                        const T* __restrict__ q, const T* __restrict__ k,
                        const T* __restrict__ wq, const T* __restrict__ wk,
@@ -386,25 +411,25 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
                        int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
                        int q_ctas, int log_lanes, RopeShape sh, unsigned* err) {
   using R = RawOf<T, VE>;
+  extern __shared__ __align__(16) unsigned char ring[];  // [stage][head][x a, x b, g a, g b][thread]
   __shared__ float sums[kVecThreads / kWarp][kMaxHeadDim];
   pdl_launch_dependents();
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
   const int dim = static_cast<int>(sh.dim);
   const bool is_q = static_cast<int>(blockIdx.x) < q_ctas;
   const int heads = static_cast<int>(is_q ? sh.q_heads : sh.k_heads);
-  const int parts = (heads + HPG - 1) / HPG;
+  const uint32_t parts = (heads + HPG - 1) / HPG;
   const int cta = is_q ? blockIdx.x : blockIdx.x - q_ctas;
   const int ctas = is_q ? q_ctas : gridDim.x - q_ctas;
   const T* x0 = is_q ? q : k;
   const T* g0 = is_q ? gq : gk;
   T* dx0 = is_q ? dq : dk;
   const int64_t x_stride = is_q ? q_stride : k_stride, g_stride = is_q ? gq_stride : gk_stride;
-  const PairPlace pl = pair_place<VE>(lane, sh);
+  const PairPlace pl = pair_place<VE, kAdjacent>(lane, sh);
   const bool holds = lane * 2 * VE < dim;
-  const uint64_t pol = evict_first_policy();
   const float inv_d = 1.f / static_cast<float>(dim);
 
-  float wa[VE], wb[VE], acc_a[VE] = {}, acc_b[VE] = {};
+  float2 wa[VE / 2], wb[VE / 2], acc_a[VE / 2] = {}, acc_b[VE / 2] = {};
   R ra = {}, rb = {};
   if (holds) {
     const T* w = is_q ? wq : wk;
@@ -414,81 +439,133 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
   unpack_raw<T, VE>(ra, wa);
   unpack_raw<T, VE>(rb, wb);
 
-  const int per_cta = kVecThreads >> log_lanes;
+  // this thread's slot of vector v of head i in a stage
+  const auto slot = [&](int stage, int i, int v) {
+    return ((stage * HPG + i) * 4 + v) * kVecThreads + static_cast<int>(threadIdx.x);
+  };
   const int64_t items = sh.tokens * parts;
-  // every lane of the CTA takes the same number of turns: the shuffles need whole warps
-  for (int64_t base = static_cast<int64_t>(cta) * per_cta; base < items;
-       base += static_cast<int64_t>(ctas) * per_cta) {
-    const int64_t item = base + (threadIdx.x >> log_lanes);
-    const bool live = item < items;
-    const int t = live ? static_cast<int>(static_cast<uint32_t>(item) / parts) : 0;
-    const int h0 = live ? (static_cast<int>(item) - t * parts) * HPG : 0;
-    const int mine = live && holds ? min(HPG, heads - h0) : 0;
-    const T* x = x0 + t * x_stride + static_cast<int64_t>(h0) * dim;
-    const T* g = g0 + t * g_stride + static_cast<int64_t>(h0) * dim;
-    R rx[HPG][2], rg[HPG][2];
+  const int64_t step = static_cast<int64_t>(ctas) * (kVecThreads >> log_lanes);
+  const int64_t first = static_cast<int64_t>(cta) * (kVecThreads >> log_lanes);
+  int64_t ahead = first + (threadIdx.x >> log_lanes);  // the item that is loaded next
+  int64_t next_pos = 0;  // its token's position is held until its turn comes
+  int64_t held_pos[kBackStages - 1];
+  const auto load = [&](int stage) {
+    if (ahead < items && holds) {
+      const uint32_t t = static_cast<uint32_t>(ahead) / parts;
+      const int h0 = static_cast<int>(static_cast<uint32_t>(ahead) - t * parts) * HPG;
+      const T* x = x0 + t * x_stride + static_cast<int64_t>(h0) * dim;
+      const T* g = g0 + t * g_stride + static_cast<int64_t>(h0) * dim;
 #pragma unroll
-    for (int i = 0; i < HPG; ++i) {
-      rx[i][0] = rx[i][1] = rg[i][0] = rg[i][1] = R{};
-      if (i < mine) {
-        rg[i][0] = load_stream<R>(g + i * dim + pl.a, pol);
-        rg[i][1] = load_stream<R>(g + i * dim + pl.b, pol);
-        rx[i][0] = load_stream<R>(x + i * dim + pl.a, pol);
-        rx[i][1] = load_stream<R>(x + i * dim + pl.b, pol);
+      for (int i = 0; i < HPG; ++i) {
+        if (h0 + i >= heads) break;
+        const T* src[4] = {x + i * dim + pl.a, x + i * dim + pl.b, g + i * dim + pl.a,
+                           g + i * dim + pl.b};
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const uint32_t dst = smem_u32(ring) + slot(stage, i, v) * static_cast<uint32_t>(sizeof(R));
+          if constexpr (sizeof(R) == 16) cp_async16(dst, src[v], true);
+          else cp_async8(dst, src[v], true);
+        }
       }
     }
-    int64_t pos = live ? positions[t] : 0;
+    cp_async_commit();
+    next_pos = ahead < items ? positions[static_cast<uint32_t>(ahead) / parts] : 0;
+    ahead += step;
+  };
+#pragma unroll
+  for (int i = 0; i < kBackStages - 1; ++i) {
+    load(i);
+    held_pos[i] = next_pos;
+  }
+
+  int stage = 0;
+  // every lane of the CTA takes the same number of turns: the shuffles need whole warps
+  for (int64_t base = first; base < items; base += step) {
+    load(stage == 0 ? kBackStages - 1 : stage - 1);
+    const int64_t item = base + (threadIdx.x >> log_lanes);
+    const bool live = item < items;
+    const uint32_t t = live ? static_cast<uint32_t>(item) / parts : 0;
+    const int h0 = live ? static_cast<int>(static_cast<uint32_t>(item) - t * parts) * HPG : 0;
+    const int mine = live && holds ? min(HPG, heads - h0) : 0;
+    int64_t pos = held_pos[0];
+#pragma unroll
+    for (int i = 0; i + 1 < kBackStages - 1; ++i) held_pos[i] = held_pos[i + 1];
+    held_pos[kBackStages - 2] = next_pos;
     const bool bad = live && (pos < 0 || pos >= sh.max_pos);
     if (bad) {
       if (lane == 0) atomicOr(err, kErrIndex);
       pos = 0;
     }
-    float c[VE], s[VE];
-    load_angles<VE>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, c, s);
+    float2 ca[VE / 2], sa[VE / 2], cb[VE / 2], sb[VE / 2];
+    load_angles<VE, kAdjacent>(cos_sin + pos * sh.rot, pl, sh, mine > 0 && !bad, ca, sa, cb, sb);
     T* dx = dx0 + (static_cast<int64_t>(t) * heads + h0) * dim;
+    cp_async_wait<kBackStages - 1>();
+    const R* held = reinterpret_cast<const R*>(ring);
 #pragma unroll
     for (int i = 0; i < HPG; ++i) {
-      float xa[VE], xb[VE], ya[VE], yb[VE], sq = 0.f, inner = 0.f;
-      unpack_raw<T, VE>(rx[i][0], xa);
-      unpack_raw<T, VE>(rx[i][1], xb);
-      unpack_raw<T, VE>(rg[i][0], ya);
-      unpack_raw<T, VE>(rg[i][1], yb);
-      if (pl.turned) turn<VE>(ya, yb, c, s, -1.f, sh.interleaved);
+      float2 xa[VE / 2], xb[VE / 2], ya[VE / 2], yb[VE / 2], sq = both(0.f), inner = both(0.f);
+      R raw[4] = {};
+      if (i < mine) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        sq = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], sq));
-        inner = fmaf(ya[e] * wa[e], xa[e], fmaf(yb[e] * wb[e], xb[e], inner));
+        for (int v = 0; v < 4; ++v) raw[v] = held[slot(stage, i, v)];
       }
-      float r = rsqrtf(group_sum(sq, lanes) * inv_d + sh.eps);
-      if (bad) r = nan_f();
-      const float m = group_sum(inner, lanes) * inv_d * r;  // mean(dn * x r)
+      unpack_raw<T, VE>(raw[0], xa);
+      unpack_raw<T, VE>(raw[1], xb);
+      unpack_raw<T, VE>(raw[2], ya);
+      unpack_raw<T, VE>(raw[3], yb);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        xa[e] *= r;
-        xb[e] *= r;
-        if (i < mine) {
-          acc_a[e] = fmaf(ya[e], xa[e], acc_a[e]);
-          acc_b[e] = fmaf(yb[e], xb[e], acc_b[e]);
+      for (int e = 0; e < VE / 2; ++e) {
+        if (pl.turned) {  // back: the sines change sign
+          const float2 ga = ya[e], gb = yb[e];
+          if constexpr (!kAdjacent) {
+            ya[e] = __ffma2_rn(gb, sa[e], __fmul2_rn(ga, ca[e]));
+            yb[e] = __ffma2_rn(neg2(ga), sa[e], __fmul2_rn(gb, ca[e]));
+          } else {
+            ya[e] = __ffma2_rn(swapped(ga), neg2(sa[e]), __fmul2_rn(ga, ca[e]));
+            yb[e] = __ffma2_rn(swapped(gb), neg2(sb[e]), __fmul2_rn(gb, cb[e]));
+          }
         }
-        xa[e] = r * fmaf(-xa[e], m, ya[e] * wa[e]);
-        xb[e] = r * fmaf(-xb[e], m, yb[e] * wb[e]);
+        sq = __ffma2_rn(xa[e], xa[e], __ffma2_rn(xb[e], xb[e], sq));
+        inner = __ffma2_rn(__fmul2_rn(ya[e], wa[e]), xa[e],
+                           __ffma2_rn(__fmul2_rn(yb[e], wb[e]), xb[e], inner));
+      }
+      const float2 sums2 = group_sum2(make_float2(sq.x + sq.y, inner.x + inner.y), lanes);
+      float r = rsqrtf(sums2.x * inv_d + sh.eps);
+      if (bad) r = nan_f();
+      // dx = r dy w - x r^2 mean(dn x r) with mean(dn x r) = r mean(dn x)
+      const float m = sums2.y * inv_d * r;
+      const float2 r2 = both(r), mr = both(-m * r);
+#pragma unroll
+      for (int e = 0; e < VE / 2; ++e) {
+        xa[e] = __fmul2_rn(xa[e], r2);
+        xb[e] = __fmul2_rn(xb[e], r2);
+        if (i < mine) {
+          acc_a[e] = __ffma2_rn(ya[e], xa[e], acc_a[e]);
+          acc_b[e] = __ffma2_rn(yb[e], xb[e], acc_b[e]);
+        }
+        xa[e] = __ffma2_rn(xa[e], mr, __fmul2_rn(__fmul2_rn(ya[e], wa[e]), r2));
+        xb[e] = __ffma2_rn(xb[e], mr, __fmul2_rn(__fmul2_rn(yb[e], wb[e]), r2));
       }
       if (i < mine) {
         store_raw<T, VE>(dx + i * dim + pl.a, xa);
         store_raw<T, VE>(dx + i * dim + pl.b, xb);
       }
     }
+    stage = stage + 1 == kBackStages ? 0 : stage + 1;
   }
+  cp_async_wait<0>();
   const int warp = threadIdx.x / kWarp;
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
+    float va = e % 2 ? acc_a[e / 2].y : acc_a[e / 2].x;
+    float vb = e % 2 ? acc_b[e / 2].y : acc_b[e / 2].x;
     for (int o = lanes; o < kWarp; o <<= 1) {
-      acc_a[e] += __shfl_xor_sync(kFull, acc_a[e], o);
-      acc_b[e] += __shfl_xor_sync(kFull, acc_b[e], o);
+      va += __shfl_xor_sync(kFull, va, o);
+      vb += __shfl_xor_sync(kFull, vb, o);
     }
     if ((threadIdx.x & (kWarp - 1)) < lanes && holds) {
-      sums[warp][pl.a + e] = acc_a[e];
-      sums[warp][pl.b + e] = acc_b[e];
+      sums[warp][pl.a + e] = va;
+      sums[warp][pl.b + e] = vb;
     }
   }
   __syncthreads();
@@ -570,9 +647,10 @@ int launch_pairs(const T* q, const T* k, const T* wq, const T* wk, const float* 
                  int64_t k_stride, const RopeShape& sh, unsigned* err, cudaStream_t s) {
   const int log = lanes_log2(sh.dim / (2 * VE));
   const int64_t items = sh.tokens * (cdiv(sh.q_heads, HPG) + cdiv(sh.k_heads, HPG));
-  rope_vector_pairs<T, VE, HPG>
-      <<<static_cast<unsigned>(cdiv(items << log, kVecThreads)), kVecThreads, 0, s>>>(
-          q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride, k_stride, log, sh, err);
+  auto* kernel = sh.interleaved ? rope_vector_pairs<T, VE, HPG, true>
+                                : rope_vector_pairs<T, VE, HPG, false>;
+  kernel<<<static_cast<unsigned>(cdiv(items << log, kRopeThreads)), kRopeThreads, 0, s>>>(
+      q, k, wq, wk, cos_sin, positions, q_out, k_out, q_stride, k_stride, log, sh, err);
   KPB_LAUNCHED("qk_norm_rope vector pairs");
   return KPB_OK;
 }
@@ -636,10 +714,13 @@ int launch_back_pairs(const T* gq, const T* gk, const T* q, const T* k, const T*
                       cudaStream_t s) {
   constexpr int HPG = 2;
   const int dim = static_cast<int>(sh.dim), log = lanes_log2(dim / (2 * VE));
-  auto* kernel = rope_back_vector_pairs<T, VE, HPG>;
+  auto* kernel = sh.interleaved ? rope_back_vector_pairs<T, VE, HPG, true>
+                                : rope_back_vector_pairs<T, VE, HPG, false>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  constexpr int kSmem = kBackStages * HPG * 4 * kVecThreads * VE * static_cast<int>(sizeof(T));
   int occ = 0;
-  if (int rc = occupancy_blocks(reinterpret_cast<const void*>(kernel), kVecThreads, 0, &occ))
-    return rc;
+  if (int rc = ensure_dyn_smem(fn, kSmem)) return rc;
+  if (int rc = occupancy_blocks(fn, kVecThreads, kSmem, &occ)) return rc;
   // one wave, shared out by the heads; no more CTAs than there is work for, nor than partials
   const int64_t wave = int64_t{occ} * sm_count(), most = back_ctas(sh, sm_count());
   const int64_t heads = sh.q_heads + sh.k_heads;
@@ -651,7 +732,7 @@ int launch_back_pairs(const T* gq, const T* gk, const T* q, const T* k, const T*
   };
   const int64_t nq = ctas_of(sh.q_heads), nk = ctas_of(sh.k_heads);
   if (nq + nk > 0) {
-    kernel<<<static_cast<unsigned>(nq + nk), kVecThreads, 0, s>>>(
+    kernel<<<static_cast<unsigned>(nq + nk), kVecThreads, kSmem, s>>>(
         gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, partials, gq_stride, gk_stride,
         q_stride, k_stride, static_cast<int>(nq), log, sh, err);
     KPB_LAUNCHED("qk_norm_rope_backward vector pairs");
