@@ -37,6 +37,14 @@ struct KvLayout {
   }
 };
 
+// log2 of n, -1 where n is no power of two.
+inline int log2_of(int64_t n) {
+  if ((n & (n - 1)) != 0) return -1;
+  int log = 0;
+  while (int64_t{1} << log < n) ++log;
+  return log;
+}
+
 __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 
 // Scale of an e4m3 row whose largest magnitude has the bit pattern `amax` (sign cleared;

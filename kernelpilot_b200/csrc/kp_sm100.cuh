@@ -102,6 +102,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                :: "r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;"
                :: "r"(dst), "l"(src), "r"(in ? 8 : 0) : "memory");

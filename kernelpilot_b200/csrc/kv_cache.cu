@@ -307,13 +307,6 @@ int lanes_log2(int64_t vectors) {
   return log;
 }
 
-int log2_of(int64_t n) {  // -1 where n is no power of two
-  if ((n & (n - 1)) != 0) return -1;
-  int log = 0;
-  while (int64_t{1} << log < n) ++log;
-  return log;
-}
-
 template <typename T, typename C>
 int launch_write(int variant, const void* k, const void* v, const int64_t* slots, void* k_cache,
                  void* v_cache, float* k_scale, float* v_scale, int64_t tokens, int64_t k_stride,

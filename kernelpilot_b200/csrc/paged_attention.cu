@@ -8,16 +8,17 @@
 //
 //   variant 0  one CTA per (sequence, query head): four warps take every fourth key each,
 //              lanes strided over the row's elements, and join at the end
-//   variant 1  the keys of all sequences split evenly over one wave of CTAs, whatever the
-//              lengths are. A unit of work is 64 keys of one row, a row being a (sequence,
-//              key head, tile of its query heads); CTA c of W takes units c * total / W to
-//              (c + 1) * total / W, found from the lengths on the device, so one captured
-//              call serves any lengths. A row that lies in one CTA is finished there; one
-//              that several CTAs share leaves a partial (maximum, sum, weighted values) per
-//              CTA, joined in CTA order by a second kernel (a programmatic dependent).
-//              Each of a CTA's four warps takes 16 of a unit's keys and streams its own
-//              keys and values, so no barrier stands between a load and its use; the warps
-//              meet once per row. Two ways to the products:
+//   variant 1  the keys of all sequences split evenly over the warps of one wave of CTAs,
+//              whatever the lengths are. A unit of work is 16 or 32 keys of one row, a row
+//              being a (sequence, key head, tile of its query heads); every worker takes as
+//              many units as any other, give or take one, found from the lengths on the
+//              device, so one captured call serves any lengths. A row that lies with one
+//              warp is finished there; of one that several share each leaves a partial
+//              (maximum, sum, weighted values), joined in order by a second kernel (a
+//              programmatic dependent). Each warp streams its own keys and values and no
+//              barrier stands in its way: with the four warps of a CTA on one row instead,
+//              meeting in shared memory at each row's end, every call took 8 us more. Two
+//              ways to the products:
 //                split_mma   fp16 / bf16 q, rows a multiple of 16 bytes on 16-byte
 //                            boundaries: cp.async into a swizzled ring per warp, mma.sync
 //                split_simt  everything else (fp32, odd head dims, odd bases)
@@ -133,9 +134,9 @@ paged_cta_head(const T* __restrict__ q, const C* __restrict__ k_cache,
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * kWarp;
 
-// How rows and units are laid out: a unit is `unit` keys of a row; rows of a sequence are (key head, tile of `tile_heads`
-// query heads), tiles innermost; a partial has tile_heads x (pitch) floats: pitch - 4
-// weighted values, then maximum and sum.
+// How rows and units are laid out: a unit is a power of two of keys of a row; rows of a
+// sequence are (key head, tile of `tile_heads` query heads), tiles innermost; a partial has
+// tile_heads x pitch floats: pitch - 4 weighted values, then maximum and sum.
 struct SplitShape {
   int64_t rows;      // rows per sequence
   int tiles;         // tiles of query heads per key head
@@ -143,8 +144,9 @@ struct SplitShape {
   int tile_heads;
   int pitch;
   int unit_log;      // log2 of the keys per unit
+  int page_log;      // log2 of the page size, -1 where it is no power of two
   int64_t* bases;    // workspace: units before each sequence (batch), then their total
-  float* partials;   // workspace: [cta][2][tile_heads][pitch]
+  float* partials;   // workspace: [worker][2][tile_heads][pitch]
 };
 
 // Units of a row of n keys.
@@ -152,13 +154,34 @@ __device__ __forceinline__ int units_of(int64_t n, const SplitShape& sp) {
   return static_cast<int>((n + (1 << sp.unit_log) - 1) >> sp.unit_log);
 }
 
-__device__ __forceinline__ int64_t first_unit(int64_t cta, int64_t ctas, int64_t total) {
-  return cta * total / ctas;
+// a / b for a >= 0, b > 0: 64-bit division takes the better part of a microsecond, and the
+// operands nearly always fit 32 bits.
+__device__ __forceinline__ int64_t div_fast(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
-// The CTA that unit u falls to (the inverse of first_unit).
-__device__ __forceinline__ int64_t cta_of_unit(int64_t u, int64_t ctas, int64_t total) {
-  return ((u + 1) * ctas - 1) / total;
+// How `total` units are dealt out: `each` to a worker and one more to the first `extra`.
+struct Deal {
+  int64_t each, extra;
+
+  __device__ __forceinline__ Deal(int64_t total, int64_t workers)
+      : each(div_fast(total, workers)), extra(total - each * workers) {}
+  __device__ __forceinline__ int64_t first(int64_t worker) const {
+    return worker * each + min(worker, extra);
+  }
+  __device__ __forceinline__ int64_t worker_of(int64_t unit) const {
+    const int64_t more = extra * (each + 1);
+    return unit < more ? div_fast(unit, each + 1) : extra + div_fast(unit - more, each);
+  }
+};
+
+// Workers of a grid: its warps, but two units to a worker at least once there are 64 workers
+// (the second unit's loads run beside the first's; a worker less is a partial less to join).
+// Never more workers than units, so that every worker of a shared row has a part of it.
+constexpr int kMinUnits = 2;
+
+__device__ __forceinline__ int64_t workers_of(int64_t ctas, int64_t total) {
+  return min(ctas * kSplitWarps, max(total / kMinUnits, min(total, int64_t{64})));
 }
 
 // A place in the list of units: sequence, row, block of keys.
@@ -181,11 +204,19 @@ struct UnitPlace {
   }
 };
 
-// This CTA's units [*begin, *end) and the place of the first. Every thread calls it;
-// `scratch` holds kSplitWarps + 3 int64. CTA 0 leaves bases and total in the workspace.
+// What find_units needs of shared memory.
+struct FindScratch {
+  int64_t warp_sum[kSplitWarps], upto[kSplitThreads];
+};
+
+// This warp's worker number, its count of units and the place of the first. Every thread
+// calls it: thread i adds up the units of the i-th run of sequences, a scan gives each run
+// its first unit, and each warp looks its own unit up among the runs. Workers are dealt out
+// over the CTAs first, so that few units spread over all SMs. CTA 0 leaves bases and total
+// in the workspace.
 __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens,
                                                 const PagedShape& sh, const SplitShape& sp,
-                                                int64_t* scratch, int64_t* begin, int64_t* end,
+                                                FindScratch* scratch, int64_t* worker, int* count,
                                                 unsigned* err) {
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
   const int64_t per = (sh.batch + kSplitThreads - 1) / kSplitThreads;
@@ -199,43 +230,47 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
     const int64_t v = __shfl_up_sync(kFull, upto, o);
     if (lane >= o) upto += v;
   }
-  if (lane == kWarp - 1) scratch[warp] = upto;
+  if (lane == kWarp - 1) scratch->warp_sum[warp] = upto;
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kSplitWarps; ++w) {
-    if (w < warp) upto += scratch[w];
-    total += scratch[w];
+    if (w < warp) upto += scratch->warp_sum[w];
+    total += scratch->warp_sum[w];
   }
-  int64_t base = upto - mine;
-  // no more CTAs than units: every CTA of a shared row then has a part of it
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total), cta = blockIdx.x;
-  *begin = cta < ctas ? first_unit(cta, ctas, total) : 0;
-  *end = cta < ctas ? first_unit(cta + 1, ctas, total) : 0;
-  const bool here = *begin < *end && *begin >= base && *begin < upto;
-  if (blockIdx.x == 0 || here) {
+  scratch->upto[threadIdx.x] = upto;
+  if (blockIdx.x == 0) {
+    int64_t base = upto - mine;
     for (int64_t b = b0; b < b1; ++b) {
-      const int64_t units = units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
-      if (blockIdx.x == 0) sp.bases[b] = base;
-      if (here && *begin >= base && *begin < base + units) {
-        scratch[kSplitWarps] = b;
-        scratch[kSplitWarps + 1] = base;
-      }
-      base += units;
+      sp.bases[b] = base;
+      base += units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) sp.bases[sh.batch] = total;
+    if (threadIdx.x == 0) sp.bases[sh.batch] = total;
   }
   __syncthreads();
+  const int64_t workers = workers_of(gridDim.x, total);
+  *worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
   UnitPlace p = {};
-  if (*begin < *end) {
-    p.b = scratch[kSplitWarps];
-    const int64_t in = *begin - scratch[kSplitWarps + 1];
+  *count = 0;
+  if (*worker >= workers) return p;
+  const Deal deal(total, workers);
+  const int64_t begin = deal.first(*worker);
+  *count = static_cast<int>(deal.first(*worker + 1) - begin);
+  // the run that holds `begin`: as many runs end at or before it
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < kSplitThreads / kWarp; ++i)
+    before += __popc(__ballot_sync(kFull, scratch->upto[i * kWarp + lane] <= begin));
+  int64_t base = before == 0 ? 0 : scratch->upto[before - 1];
+  for (p.b = before * per;; ++p.b) {
     p.n = static_cast<int>(keys_of(seq_lens, p.b, sh, err));
     p.blocks = units_of(p.n, sp);
-    p.row = in / p.blocks;
-    p.blk = static_cast<int>(in - p.row * p.blocks);
+    const int64_t units = p.blocks * sp.rows;
+    if (begin < base + units) break;
+    base += units;
   }
-  __syncthreads();
+  p.row = div_fast(begin - base, p.blocks);
+  p.blk = static_cast<int>(begin - base - p.row * p.blocks);
   return p;
 }
 
@@ -250,103 +285,90 @@ __device__ __forceinline__ void zero_empty(T* __restrict__ o, const int* __restr
   }
 }
 
-// Joins the warps' parts of the segment that ends here (maximum s_m and sum s_l,
-// [warp][head]; weighted values s_o, [warp][head - h0][pitch], of heads h0 to h0 + held of
-// the tile) and writes it: the output where the segment is a whole row, else partial `slot`
-// of this CTA.
-template <typename T>
-__device__ __forceinline__ void write_segment(const float* s_m, const float* s_l,
-                                              const float* s_o, int h0, int held,
-                                              const UnitPlace& p, bool whole, int slot,
-                                              T* __restrict__ o, const PagedShape& sh,
-                                              const SplitShape& sp) {
-  const int64_t hk = p.row / sp.tiles;
-  const int first = static_cast<int>(p.row - hk * sp.tiles) * sp.tile_heads;
-  const int h1 = min(h0 + held, sp.group - first);
-  const int dim = static_cast<int>(sh.lay.dim);
-  for (int h = h0; h < h1; ++h) {
-    float f[kSplitWarps], top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, s_m[w * sp.tile_heads + h]);
-    const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) {
-      f[w] = ex2f(s_m[w * sp.tile_heads + h] - base);
-      sum = fmaf(f[w], s_l[w * sp.tile_heads + h], sum);
-    }
-    float* part = sp.partials +
-                  ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * sp.tile_heads + h) * sp.pitch;
-    for (int i = threadIdx.x; i < dim; i += kSplitThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w)
-        v = fmaf(f[w], s_o[(w * held + h - h0) * sp.pitch + i], v);
-      if (whole) {
-        o[(p.b * sh.q_heads + hk * sp.group + first + h) * dim + i] = from_f<T>(v / sum);
-      } else {
-        part[i] = v;
-      }
-    }
-    if (!whole && threadIdx.x == 0) {
-      part[sp.pitch - 4] = top;
-      part[sp.pitch - 3] = sum;
-    }
-  }
+// Partial `slot` (0: of a row that began before this worker, 1: of one that did not) of a
+// worker, head h of the tile.
+__device__ __forceinline__ float* partial_at(const SplitShape& sp, int64_t worker, int slot,
+                                             int h) {
+  return sp.partials + ((worker * 2 + slot) * sp.tile_heads + h) * sp.pitch;
 }
 
-// One CTA per row that several CTAs share, one warp per query head at a time, lanes
-// strided over the values: out = sum_c f_c O_c / sum_c f_c l_c over the row's partials in
-// CTA order, f_c = 2^(m_c - max m). `ctas` is the first kernel's grid.
-constexpr int kJoinWarps = 8;
+// The partials of a (sequence, query head) whose row several workers share, joined by
+// 2^share_log of a CTA's warps: each takes every so manieth partial, lanes strided over the
+// values, as out = sum_c f_c O_c / sum_c f_c l_c, f_c = 2^(m_c - max m) carried along as a
+// running maximum; then the warps in order. `ctas` is the first kernel's grid.
+constexpr int kJoinWarps = 16;
 
-template <typename T>
+template <typename T, int E>
 __global__ void __launch_bounds__(kJoinWarps * kWarp)
 join_rows(const int* __restrict__ seq_lens, T* __restrict__ o, PagedShape sh, SplitShape sp,
-          int64_t ctas, unsigned* err) {
+          int64_t ctas, int share_log, unsigned* err) {
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][E * kWarp];
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
-  const int64_t b = blockIdx.x / sp.rows, row = blockIdx.x - b * sp.rows;
+  const int share = 1 << share_log, part = warp & (share - 1), first_warp = warp - part;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kJoinWarps >> share_log) + (warp >> share_log);
+  const bool live = at < sh.batch * sh.q_heads;
+  const int64_t b = live ? div_fast(at, sh.q_heads) : 0;
+  const int head = live ? static_cast<int>(at - b * sh.q_heads) : 0;
   const int64_t blocks = units_of(keys_of(seq_lens, b, sh, err), sp);
+  const int hk = head / sp.group, g = head - hk * sp.group;
+  const int tile = g / sp.tile_heads;
   pdl_wait_primary();
   const int64_t total = sp.bases[sh.batch], base = sp.bases[b];
-  if (blocks < 2) return;
-  ctas = min(ctas, total);
-  const int64_t u0 = base + row * blocks;
-  const int64_t c0 = cta_of_unit(u0, ctas, total), c1 = cta_of_unit(u0 + blocks - 1, ctas, total);
-  if (c0 == c1) return;
-  const int64_t hk = row / sp.tiles;
-  const int first = static_cast<int>(row - hk * sp.tiles) * sp.tile_heads;
-  const int heads = min(sp.tile_heads, sp.group - first);
-  const int dim = static_cast<int>(sh.lay.dim);
-  const int count = static_cast<int>(c1 - c0) + 1;
-  // only the first CTA's segment may start inside its range (slot 1)
-  const int slot0 = u0 > first_unit(c0, ctas, total) ? 1 : 0;
-  const int64_t step = static_cast<int64_t>(2) * sp.tile_heads * sp.pitch;
-  for (int h = warp; h < heads; h += kJoinWarps) {
-    const float* p0 = sp.partials + ((c0 * 2 + slot0) * sp.tile_heads + h) * sp.pitch;
-    const float* rest = sp.partials + (c0 * 2 * sp.tile_heads + h) * sp.pitch;
-    float top = -INFINITY;
-    for (int c = lane; c < count; c += kWarp)
-      top = fmaxf(top, (c == 0 ? p0 : rest + c * step)[sp.pitch - 4]);
-    top = warp_max(top);
-    if (top == -INFINITY) top = 0.f;
-    float sum = 0.f, acc[kPerLane] = {};
+  int count = 0;
+  float m = -INFINITY, l = 0.f, acc[E] = {};
+  if (live && blocks > 1) {
+    const int64_t workers = workers_of(ctas, total);
+    const int64_t u0 = base + (static_cast<int64_t>(hk) * sp.tiles + tile) * blocks;
+    const Deal deal(total, workers);
+    const int64_t w0 = deal.worker_of(u0);
+    count = static_cast<int>(deal.worker_of(u0 + blocks - 1) - w0) + 1;
+    if (count > 1) {
+      // only the first worker's part may begin inside its units (slot 1)
+      const int h = g - tile * sp.tile_heads;
+      const float* p0 = partial_at(sp, w0, u0 > deal.first(w0) ? 1 : 0, h);
+      const float* rest = partial_at(sp, w0, 0, h);
+      const int64_t step = static_cast<int64_t>(2) * sp.tile_heads * sp.pitch;
 #pragma unroll 4
-    for (int c = 0; c < count; ++c) {
-      const float* p = c == 0 ? p0 : rest + c * step;
-      const float f = ex2f(p[sp.pitch - 4] - top);
-      sum = fmaf(f, p[sp.pitch - 3], sum);
+      for (int c = part; c < count; c += share) {
+        const float* p = c == 0 ? p0 : rest + c * step;
+        float v[E];
 #pragma unroll
-      for (int e = 0; e < kPerLane; ++e) {
-        const int i = lane + e * kWarp;
-        if (i < dim) acc[e] = fmaf(f, p[i], acc[e]);
+        for (int e = 0; e < E; ++e) v[e] = p[lane + e * kWarp];
+        const float pm = p[E * kWarp], pl = p[E * kWarp + 1];
+        const float top = fmaxf(m, pm), to = top == -INFINITY ? 0.f : top;
+        const float f = ex2f(m - to), pf = ex2f(pm - to);
+        l = fmaf(l, f, pl * pf);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], f, v[e] * pf);
+        m = top;
       }
     }
-    T* out = o + (b * sh.q_heads + hk * sp.group + first + h) * dim;
+  }
+  if (share > 1) {
 #pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      const int i = lane + e * kWarp;
-      if (i < dim) out[i] = from_f<T>(acc[e] / sum);
+    for (int e = 0; e < E; ++e) s_o[warp][lane + e * kWarp] = acc[e];
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = l;
     }
+    __syncthreads();
+    if (part != 0) return;
+    for (int w = first_warp + 1; w < first_warp + share; ++w) {
+      const float top = fmaxf(m, s_m[w]), to = top == -INFINITY ? 0.f : top;
+      const float f = ex2f(m - to), pf = ex2f(s_m[w] - to);
+      l = fmaf(l, f, s_l[w] * pf);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], f, s_o[w][lane + e * kWarp] * pf);
+      m = top;
+    }
+  }
+  if (count < 2) return;
+  const int dim = static_cast<int>(sh.lay.dim);
+  T* out = o + (b * sh.q_heads + head) * dim;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = lane + e * kWarp;
+    if (i < dim) out[i] = from_f<T>(acc[e] / l);
   }
 }
 
@@ -369,7 +391,7 @@ __device__ __forceinline__ int64_t key_row(const int* __restrict__ table, int64_
 
 // ------------------------------------------------------------------ variant 1: split_simt
 
-constexpr int kSimtUnit = 64;
+constexpr int kSimtUnit = 16;
 
 // Lanes are strided over a row's elements (E each); a warp takes 4 keys at a time and HG
 // query heads: 4 * HG products, summed over the lanes by halving, so that each lane ends
@@ -380,28 +402,25 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
            const int* __restrict__ table, const int* __restrict__ seq_lens,
            const float* __restrict__ k_scale, const float* __restrict__ v_scale,
            T* __restrict__ o, PagedShape sh, SplitShape sp, unsigned* err) {
-  constexpr int kKeys = 4, kWarpKeys = kSimtUnit / kSplitWarps;
+  constexpr int kKeys = 4;
   constexpr int kSums = kKeys * HG;
   constexpr int kLog = kSums == 32 ? 5 : kSums == 16 ? 4 : kSums == 8 ? 3 : 2;
   constexpr int kSpread = 5 - kLog;  // 2^kSpread neighbouring lanes hold the same sum
   constexpr bool kQuant = std::is_same_v<C, uint8_t>;
-  constexpr int kPitch = E * kWarp + 4;
-  __shared__ float s_m[kSplitWarps * HG], s_l[kSplitWarps * HG];
-  __shared__ float s_o[kSplitWarps * HG * kPitch];
-  __shared__ int64_t scratch[kSplitWarps + 2];
-  const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
+  __shared__ FindScratch scratch;
+  const int lane = threadIdx.x & (kWarp - 1);
   const int dim = static_cast<int>(sh.lay.dim);
   pdl_launch_dependents();
-  zero_empty(o, seq_lens, sh, err);
-  int64_t u, end;
-  UnitPlace p = find_units(seq_lens, sh, sp, scratch, &u, &end, err);
+  int64_t worker;
+  int count;
+  UnitPlace p = find_units(seq_lens, sh, sp, &scratch, &worker, &count, err);
   const int my_key = (lane >> kSpread) / HG;
 
   float qr[HG][E], acc[HG][E], m = -INFINITY, l = 0.f;
   bool fresh = true, whole_start = p.blk == 0;
   int slot = 0;
-  for (; u < end; ++u) {
-    const int64_t hk = p.row / sp.tiles;
+  for (; count > 0; --count) {
+    const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
     const int first = static_cast<int>(p.row - hk * sp.tiles) * HG;
     if (fresh) {
 #pragma unroll
@@ -418,9 +437,9 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       l = 0.f;
       fresh = false;
     }
-    const int key0 = p.blk * kSimtUnit + warp * kWarpKeys;
+    const int key0 = p.blk * kSimtUnit;
     int64_t my_scale = 0;
-    const int64_t my_row = lane < kWarpKeys
+    const int64_t my_row = lane < kSimtUnit
                                ? key_row(table, p.b, key0 + lane, p.n, hk, sh, &my_scale, err)
                                : -1;
     if (__any_sync(kFull, my_row == -2)) l = nan_f();
@@ -432,7 +451,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       }
     }
 #pragma unroll 1
-    for (int j = 0; j < kWarpKeys && key0 + j < p.n; j += kKeys) {
+    for (int j = 0; j < kSimtUnit && key0 + j < p.n; j += kKeys) {
       float kv[kKeys][E], vv[kKeys][E];
       int64_t row[kKeys];
 #pragma unroll
@@ -506,31 +525,37 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       }
     }
     const bool row_ends = p.blk + 1 == p.blocks;
-    if (row_ends || u + 1 == end) {
+    if (row_ends || count == 1) {
       float sum = l;
 #pragma unroll
       for (int off = HG << kSpread; off < kWarp; off <<= 1)
         sum += __shfl_xor_sync(kFull, sum, off);
-      const int h = (lane >> kSpread) % HG;
-      if (lane == h << kSpread) {
-        s_m[warp * HG + h] = m;
-        s_l[warp * HG + h] = sum;
-      }
+      const bool whole = whole_start && row_ends;
 #pragma unroll
-      for (int hh = 0; hh < HG; ++hh) {
+      for (int h = 0; h < HG; ++h) {
+        const float hs = __shfl_sync(kFull, sum, h << kSpread);
+        const float hm = __shfl_sync(kFull, m, h << kSpread);
+        if (first + h >= sp.group) break;
+        T* out = o + (p.b * sh.q_heads + hk * sp.group + first + h) * dim;
+        float* part = partial_at(sp, worker, slot, h);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          s_o[(warp * HG + hh) * kPitch + lane + e * kWarp] = acc[hh][e];
+        for (int e = 0; e < E; ++e) {
+          const int i = lane + e * kWarp;
+          if (!whole) part[i] = acc[h][e];
+          else if (i < dim) out[i] = from_f<T>(acc[h][e] / hs);
+        }
+        if (!whole && lane == 0) {
+          part[E * kWarp] = hm;
+          part[E * kWarp + 1] = hs;
+        }
       }
-      __syncthreads();
-      write_segment(s_m, s_l, s_o, 0, HG, p, whole_start && row_ends, slot, o, sh, sp);
-      __syncthreads();
       fresh = true;
       whole_start = true;
       slot = 1;
     }
     p.next(seq_lens, sh, sp, err);
   }
+  zero_empty(o, seq_lens, sh, err);
 }
 
 // ------------------------------------------------------------------ variant 1: split_mma
@@ -571,22 +596,28 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
-// Weights w >= 0 as a pair of M (x in the low half) cut towards zero, and as *rest what that
-// leaves. The rest is never 0 beside a weight that is not: an infinite value times the pair
-// is then an infinity, not infinity * 0.
-template <typename M>
+// Weights w >= 0 as a pair of M (x in the low half), and as *rest what that leaves. Where
+// the values may hold infinities (kCut: not e4m3 codes) the pair is cut towards zero and the
+// rest is never 0 beside a weight that is not: an infinite value times the two is then an
+// infinity, not infinity * 0 or the difference of two.
+template <typename M, bool kCut>
 __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* rest) {
   constexpr float kTiny = 1.f / (1 << 24);
   uint32_t hi;
   float2 f;
   if constexpr (std::is_same_v<M, __half>) {
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    if constexpr (kCut) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
     f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   } else {
     asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
     f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi));
   }
-  const float rx = fmaxf(x - f.x, fminf(x, kTiny)), ry = fmaxf(y - f.y, fminf(y, kTiny));
+  float rx = x - f.x, ry = y - f.y;
+  if constexpr (kCut) {
+    rx = fmaxf(rx, fminf(x, kTiny));
+    ry = fmaxf(ry, fminf(y, kTiny));
+  }
   if constexpr (std::is_same_v<M, __half>) {
     const __half2 v = __floats2half2_rn(rx, ry);
     *rest = *reinterpret_cast<const uint32_t*>(&v);
@@ -601,10 +632,13 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
 // fraction down to 2^-28 of the largest weight and something down to 2^-38.
 constexpr float kWeightBits = 14.f;
 
-// Two e4m3 codes (the low 16 bits) as a pair of fp16, exactly.
-__device__ __forceinline__ uint32_t codes_to_half(uint32_t w) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+// Four e4m3 codes as two pairs of fp16, exactly.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* lo, uint32_t* hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(*lo), "=r"(*hi) : "r"(w));
 }
 
 // Byte offset of 16-byte chunk `ch` of row `row` in a tile of rows of kRow bytes, chunks
@@ -618,27 +652,31 @@ __device__ __forceinline__ uint32_t tile_at(int row, int ch) {
   }
 }
 
-// Shared memory of one CTA: kStages x (keys, values, scales) per warp, then the warps'
-// meeting place, kMeetHeads heads at a time. A warp takes 32 keys at a time where a row is
-// 128 bytes at most, else 16. As many stages as let three CTAs share an SM, two at least
-// and four at most; with two that do not fit, two CTAs or one.
-constexpr int kMeetHeads = 4;
+// tile_at(row0 + lr, ch) for a constant row0 and lr < the rows of a turn (which divide 8, or
+// are 8): the exchange splits into a constant part and one that stays.
+template <int kRow>
+__device__ __forceinline__ uint32_t tile_turn(int row0, int lr, int ch) {
+  const uint32_t mine = static_cast<uint32_t>(
+      lr * kRow + ((ch ^ (kRow >= 128 ? lr : lr >> 1 & 3)) << 4));
+  return row0 * kRow + (mine ^ static_cast<uint32_t>(kRow >= 128 ? (row0 & 7) << 4 : 0));
+}
 
+// Shared memory of one CTA: kStages x (keys, values, scales) per warp. A warp takes 32 keys
+// at a time where a row is 128 bytes at most, else 16. As many stages as let three CTAs
+// share an SM, two at least and four at most; where two do not fit, two CTAs or one.
 template <typename C, int DP, int NT>
 struct MmaPlan {
   static constexpr bool kQuant = std::is_same_v<C, uint8_t>;
   static constexpr int kRow = DP * static_cast<int>(sizeof(C));
   static constexpr int kKeys = kRow <= 128 && DP * NT <= 128 ? 32 : 16;
-  static constexpr int kUnit = kSplitWarps * kKeys;
   static constexpr int kTile = kKeys * kRow;
   static constexpr int kStage = 2 * kTile + (kQuant ? 2 * kKeys * 4 : 0);
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPitch = DP + 4;
-  static constexpr int kMeet = kSplitWarps * (2 * kHeads + kMeetHeads * kPitch) * 4 + 64;
-  static constexpr int kThirdSm = 228 * 1024 / 3 - 1024;
-  static constexpr int kFit = (kThirdSm - kMeet) / (kSplitWarps * kStage);
+  static constexpr int kScratch = static_cast<int>(sizeof(FindScratch));
+  static constexpr int kFit = (228 * 1024 / 3 - 1024 - kScratch) / (kSplitWarps * kStage);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
-  static constexpr int kSmem = kSplitWarps * kStages * kStage + kMeet;
+  static constexpr int kSmem = kSplitWarps * kStages * kStage + kScratch;
 };
 
 // Rows of the cache as the loader holds them: 16-byte units from the cache's start, in 32
@@ -654,9 +692,10 @@ constexpr uint32_t kBadRow = 0xfffffffeu;  // in a page outside the cache
 // weights enter as two 16-bit parts (split_weights), so that they carry 2^-15 of themselves
 // (bf16) or 2^-21 (fp16); the second product is a small part of the time that loading takes.
 // e4m3: codes become fp16 in registers, q is scaled by a power of two to [1, 2) (exact) and
-// the key's scale multiplies its score. The value's scale goes into the weight in log2
-// before the exponential, with a maximum of its own, so that a weight times its scale stays
-// within fp16 whatever the scales are.
+// the key's scale multiplies its score. The value's scale multiplies the weight, relative to
+// the power of two above the largest scale that the warp has met (the running sums follow
+// when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's full
+// fraction while its scale is above 2^-28 of the largest.
 template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(kSplitThreads)
 split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __restrict__ v_cache,
@@ -670,36 +709,35 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   constexpr int kKeys = Plan::kKeys, kTiles = kKeys / 16;
   constexpr int kChunks = kRow / 16;
   constexpr int kSteps = DP / 16;
+  constexpr int kRows = kWarp / kChunks, kTurns = kKeys / kRows;
   extern __shared__ __align__(128) unsigned char smem[];
-  float* s_m = reinterpret_cast<float*>(smem + kSplitWarps * kS * Plan::kStage);
-  float* s_l = s_m + kSplitWarps * kHeads;
-  float* s_o = s_l + kSplitWarps * kHeads;
-  auto* scratch = reinterpret_cast<int64_t*>(s_o + kSplitWarps * kMeetHeads * Plan::kPitch);
+  auto* scratch = reinterpret_cast<FindScratch*>(smem + kSplitWarps * kS * Plan::kStage);
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
   const int r = lane >> 2, t = lane & 3;  // row and column pair of this lane's fragments
   const int dim = static_cast<int>(sh.lay.dim);
   const uint32_t ring = smem_u32(smem) + warp * kS * Plan::kStage;
   const int chunks_in = dim * static_cast<int>(sizeof(C)) / 16;
+  const int lr = lane / kChunks, ch = lane % kChunks;  // the loader's row of a turn, and chunk
 
   pdl_launch_dependents();
-  zero_empty(o, seq_lens, sh, err);
-  int64_t u, end;
-  UnitPlace p = find_units(seq_lens, sh, sp, scratch, &u, &end, err);
-  if (u >= end) return;
+  int64_t worker;
+  int count;
+  UnitPlace p = find_units(seq_lens, sh, sp, scratch, &worker, &count, err);
 
   // The loader runs kS - 1 units ahead, and looks up its next unit's pages one unit before
   // that: next_row / next_scale are those of this lane's key (lane % kKeys).
   UnitPlace lp = p;
-  int left = static_cast<int>(end - u);  // units that the loader has not begun
+  int left = count;  // units that the loader has not begun
   uint32_t next_row = kNoRow, next_scale = 0;
   unsigned bad_slots = 0;
   const auto page_size = static_cast<uint32_t>(sh.lay.page_size);
   const auto page_units = static_cast<uint32_t>(sh.lay.page_stride * sizeof(C) / 16);
   auto look_up = [&]() {
     next_row = kNoRow;
-    const uint32_t pos = lp.blk * Plan::kUnit + warp * kKeys + (lane & (kKeys - 1));
+    const uint32_t pos = lp.blk * kKeys + (lane & (kKeys - 1));
     if (left <= 0 || pos >= static_cast<uint32_t>(lp.n)) return;
-    const uint32_t at = pos / page_size, off = pos - at * page_size;
+    const uint32_t at = sp.page_log >= 0 ? pos >> sp.page_log : pos / page_size;
+    const uint32_t off = pos - at * page_size;
     const int page = table[lp.b * sh.table_stride + at];
     if (page < 0 || page >= sh.lay.num_pages) {
       atomicOr(err, kErrIndex);
@@ -715,15 +753,27 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
       const uint32_t kd = ring + stage * Plan::kStage, vd = kd + Plan::kTile;
       const bool bad = __any_sync(kFull, next_row == kBadRow);
       bad_slots = bad ? bad_slots | (1u << stage) : bad_slots & ~(1u << stage);
+      // a turn copies kRows rows, each lane a chunk of one; whole tiles without the marks
+      const uint64_t lane_byte = static_cast<uint64_t>(ch) * 16;
+      if (__all_sync(kFull, next_row < kBadRow) && chunks_in == kChunks) {
 #pragma unroll
-      for (int i = 0; i < kKeys * kChunks / kWarp; ++i) {
-        const int c = i * kWarp + lane;
-        const int row = c / kChunks, ch = c % kChunks;
-        const uint32_t at = __shfl_sync(kFull, next_row, row);
-        const bool in = at < kBadRow && ch < chunks_in;
-        const uint64_t byte = in ? static_cast<uint64_t>(at + ch) * 16 : 0;
-        cp_async16(kd + tile_at<kRow>(row, ch), reinterpret_cast<const char*>(k_cache) + byte, in);
-        cp_async16(vd + tile_at<kRow>(row, ch), reinterpret_cast<const char*>(v_cache) + byte, in);
+        for (int i = 0; i < kTurns; ++i) {
+          const uint64_t byte =
+              static_cast<uint64_t>(__shfl_sync(kFull, next_row, i * kRows + lr)) * 16 + lane_byte;
+          const uint32_t at = tile_turn<kRow>(i * kRows, lr, ch);
+          cp_async16(kd + at, reinterpret_cast<const char*>(k_cache) + byte);
+          cp_async16(vd + at, reinterpret_cast<const char*>(v_cache) + byte);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          const uint32_t row = __shfl_sync(kFull, next_row, i * kRows + lr);
+          const bool in = row < kBadRow && ch < chunks_in;
+          const uint64_t byte = in ? static_cast<uint64_t>(row) * 16 + lane_byte : 0;
+          const uint32_t at = tile_turn<kRow>(i * kRows, lr, ch);
+          cp_async16(kd + at, reinterpret_cast<const char*>(k_cache) + byte, in);
+          cp_async16(vd + at, reinterpret_cast<const char*>(v_cache) + byte, in);
+        }
       }
       if constexpr (kQuant) {  // the key scales, then the value scales
         const bool in = next_row < kBadRow;
@@ -747,13 +797,14 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   uint32_t qb[NT][kSteps][2];
   float mult[NT][2];                      // score -> log2 units, heads 2t and 2t + 1
   float acc[NT][kSteps][4];               // O^T: elements x heads
-  float m[NT][2], l[NT][2], mo[NT][2];    // running maximum, sum; maximum of weight * scale
+  float m[NT][2], l[NT][2];               // running maximum and sum
+  uint32_t vref = 1;                      // e4m3: exponent that value scales are relative to
   bool fresh = true, whole_start = p.blk == 0;
   int slot = 0, stage = 0;
-  for (int units = static_cast<int>(end - u); units > 0; --units) {
+  for (; count > 0; --count) {
     if (fresh) {
       fresh = false;
-      const int64_t hk = p.row / sp.tiles;
+      const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
       const int first = static_cast<int>(p.row - hk * sp.tiles) * kHeads;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -812,20 +863,23 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[nt][kk][i] = 0.f;
         }
-        m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
       }
+      vref = 1;
     }
 
     load(stage == 0 ? kS - 1 : stage - 1);
     cp_async_wait<kS - 1>();
     __syncwarp();
     const uint32_t kt = ring + stage * Plan::kStage, vt = kt + Plan::kTile;
-    const int key0 = p.blk * Plan::kUnit + warp * kKeys;
-    if (key0 < p.n) {  // else none of this warp's keys is left in the row
+    const int key0 = p.blk * kKeys;
+    {
       // scores: block l / 8 of an ldmatrix is keys (l / 8) % 2 * 8 .., chunk + l / 16
       const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
-      float c[kTiles][NT][2][4] = {};
+      // two chains of sums where a single 16-key tile would leave one
+      constexpr int kChains = kTiles * NT > 1 ? 1 : 2;
+      float c[kTiles][NT][kChains][4] = {};
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         if constexpr (!kQuant) {
@@ -835,7 +889,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
             ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, 2 * kk + kch), a);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<M>(c[j][nt][kk & 1], a[0], a[1], a[2], a[3], qb[nt][kk][0], qb[nt][kk][1]);
+              mma16816<M>(c[j][nt][kk % kChains], a[0], a[1], a[2], a[3], qb[nt][kk][0], qb[nt][kk][1]);
           }
         } else {
 #pragma unroll
@@ -844,26 +898,36 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
             ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t a0 = codes_to_half(w[2 * i]), a1 = codes_to_half(w[2 * i + 1]);
-              const uint32_t a2 = codes_to_half(w[2 * i] >> 16);
-              const uint32_t a3 = codes_to_half(w[2 * i + 1] >> 16);
+              uint32_t a0, a1, a2, a3;
+              codes_to_half(w[2 * i], &a0, &a2);
+              codes_to_half(w[2 * i + 1], &a1, &a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma16816<M>(c[j][nt][i], a0, a1, a2, a3, qb[nt][kk + i][0], qb[nt][kk + i][1]);
+                mma16816<M>(c[j][nt][i % kChains], a0, a1, a2, a3, qb[nt][kk + i][0], qb[nt][kk + i][1]);
             }
           }
         }
       }
-      float ks[kTiles][2], vlog[kTiles][2];
+      float ks[kTiles][2], vs[kTiles][2], shrink = 1.f;
       if constexpr (kQuant) {
         const float* sc = reinterpret_cast<const float*>(
             smem + (warp * kS + stage) * Plan::kStage + 2 * Plan::kTile);
+        // the exponent above the largest finite value scale (positive: ordered as integers);
+        // past the last key the scale's place holds 0
+        const uint32_t mine = __float_as_uint(sc[kKeys + (lane & (kKeys - 1))]);
+        const uint32_t top =
+            min((__reduce_max_sync(kFull, mine >= 0x7f800000u ? 0u : mine) >> 23) + 1, 253u);
+        if (top > vref) {  // the sums so far become relative to the new one
+          shrink = exp2f(static_cast<float>(static_cast<int>(vref) - static_cast<int>(top)));
+          vref = top;
+        }
+        const float down = __uint_as_float((254 - vref) << 23);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             ks[j][h] = sc[16 * j + 8 * h + r];
-            vlog[j][h] = __log2f(sc[kKeys + 16 * j + 8 * h + r]);
+            vs[j][h] = sc[kKeys + 16 * j + 8 * h + r] * down;
           }
         }
       }
@@ -874,55 +938,38 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
         float w[kTiles][2][2], alpha[2];  // [16 keys][key r, r + 8][head 2t, 2t + 1]
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = -INFINITY, vtop = -INFINITY;
+          float top = -INFINITY;
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float s = c[j][nt][0][2 * h + i] + c[j][nt][1][2 * h + i];
+              float s = c[j][nt][0][2 * h + i];
+              if constexpr (kChains == 2) s += c[j][nt][1][2 * h + i];
               s *= kQuant ? mult[nt][i] * ks[j][h] : mult[nt][i];
               if (!full && key0 + 16 * j + 8 * h + r >= p.n) s = -INFINITY;
               w[j][h][i] = s;
               top = fmaxf(top, s);
-              // past the last key the scale's place holds 0: log2 gives -inf there
-              if constexpr (kQuant) vtop = fmaxf(vtop, s + vlog[j][h]);
             }
           }
 #pragma unroll
-          for (int off = 4; off < kWarp; off <<= 1) {
+          for (int off = 4; off < kWarp; off <<= 1)
             top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-            if constexpr (kQuant) vtop = fmaxf(vtop, __shfl_xor_sync(kFull, vtop, off));
-          }
           const float m_new = fmaxf(m[nt][i], top);
           const float base = m_new == -INFINITY ? 0.f : m_new;
           alpha[i] = ex2f(m[nt][i] - base);
           float sum = 0.f;
-          if constexpr (kQuant) {
-            const float mo_new = fmaxf(mo[nt][i], vtop);
-            const float vbase = mo_new == -INFINITY ? 0.f : mo_new;
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
+          for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                sum += ex2f(w[j][h][i] - (base - kWeightBits));
-                w[j][h][i] = ex2f(w[j][h][i] + vlog[j][h] - (vbase - kWeightBits));
-              }
+            for (int h = 0; h < 2; ++h) {
+              w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
+              sum += w[j][h][i];
+              if constexpr (kQuant) w[j][h][i] *= vs[j][h];
             }
-            l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
-            alpha[i] = ex2f(mo[nt][i] - vbase);
-            mo[nt][i] = mo_new;
-          } else {
-#pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
-                sum += w[j][h][i];
-              }
-            }
-            l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
           }
+          l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
           m[nt][i] = m_new;
+          if constexpr (kQuant) alpha[i] *= shrink;
         }
         if (__any_sync(kFull, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -936,7 +983,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t rest;
-            hi[j][nt][h] = transpose8(split_weights<M>(w[j][h][0], w[j][h][1], &rest));
+            hi[j][nt][h] = transpose8(split_weights<M, !kQuant>(w[j][h][0], w[j][h][1], &rest));
             lo[j][nt][h] = transpose8(rest);
           }
         }
@@ -966,10 +1013,9 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               // bytes: key 2t (two elements), key 2t + 1 (two) -> element by element
-              const uint32_t x = __byte_perm(w[2 * i], 0, 0x3120);
-              const uint32_t y = __byte_perm(w[2 * i + 1], 0, 0x3120);
-              const uint32_t a0 = codes_to_half(x), a1 = codes_to_half(x >> 16);
-              const uint32_t a2 = codes_to_half(y), a3 = codes_to_half(y >> 16);
+              uint32_t a0, a1, a2, a3;
+              codes_to_half(__byte_perm(w[2 * i], 0, 0x3120), &a0, &a1);
+              codes_to_half(__byte_perm(w[2 * i + 1], 0, 0x3120), &a2, &a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, hi[j][nt][0], hi[j][nt][1]);
@@ -988,9 +1034,10 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     stage = stage + 1 == kS ? 0 : stage + 1;
 
     const bool row_ends = p.blk + 1 == p.blocks;
-    if (row_ends || units == 1) {
-      const int heads = min(kHeads, sp.group - static_cast<int>(p.row % sp.tiles) * kHeads);
-      float f[NT][2];
+    if (row_ends || count == 1) {
+      const bool whole = whole_start && row_ends;
+      const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
+      const int first = static_cast<int>(p.row - hk * sp.tiles) * kHeads;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -998,35 +1045,29 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           float sum = l[nt][i];
 #pragma unroll
           for (int off = 4; off < kWarp; off <<= 1) sum += __shfl_xor_sync(kFull, sum, off);
-          if (r == 0) {
-            s_m[warp * kHeads + nt * 8 + 2 * t + i] = m[nt][i];
-            s_l[warp * kHeads + nt * 8 + 2 * t + i] = sum;
-          }
-          // values of e4m3 rows are relative to the other maximum
-          f[nt][i] = 1.f;
-          if constexpr (kQuant)
-            f[nt][i] = mo[nt][i] == -INFINITY ? 1.f : ex2f(mo[nt][i] - m[nt][i]);
-        }
-      }
+          const int h = nt * 8 + 2 * t + i;
+          if (first + h < sp.group) {
+            // values of e4m3 rows are relative to 2^(vref - 127)
+            float f = kQuant ? __uint_as_float(vref << 23) : 1.f;
+            if (whole) f /= sum;
+            T* out = o + (p.b * sh.q_heads + hk * sp.group + first + h) * dim;
+            float* part = partial_at(sp, worker, slot, h);
+            if (!whole && r == 0) {
+              part[DP] = m[nt][i];
+              part[DP + 1] = sum;
+            }
 #pragma unroll
-      for (int h0 = 0; h0 < kHeads; h0 += kMeetHeads) {
-        if (h0 >= heads) break;
-        const int nt = h0 / 8, at_t = t - (h0 % 8) / 2;  // this round's heads: nt, t of 0 .. 1
-        if (at_t == 0 || at_t == 1) {
+            for (int kk = 0; kk < kSteps; ++kk) {
 #pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-            const int d0 = kk * 16 + (kQuant ? 2 * r : r), d1 = d0 + (kQuant ? 1 : 8);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float* at = s_o + (warp * kMeetHeads + 2 * at_t + i) * Plan::kPitch;
-              at[d0] = acc[nt][kk][i] * f[nt][i];
-              at[d1] = acc[nt][kk][2 + i] * f[nt][i];
+              for (int j = 0; j < 2; ++j) {
+                const int d = kk * 16 + (kQuant ? 2 * r + j : r + 8 * j);
+                const float v = acc[nt][kk][2 * j + i] * f;
+                if (!whole) part[d] = v;
+                else if (d < dim) out[d] = from_f<T>(v);
+              }
             }
           }
         }
-        __syncthreads();
-        write_segment(s_m, s_l, s_o, h0, kMeetHeads, p, whole_start && row_ends, slot, o, sh, sp);
-        __syncthreads();
       }
       fresh = true;
       whole_start = true;
@@ -1035,6 +1076,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     p.next(seq_lens, sh, sp, err);
   }
   cp_async_wait<0>();
+  zero_empty(o, seq_lens, sh, err);
 }
 
 // ------------------------------------------------------------------ launch
@@ -1048,9 +1090,6 @@ struct PagedCall {
   unsigned* err;
   cudaStream_t s;
 };
-
-// The widest grid: what bounds a call's partials, two per CTA of tile_heads x pitch floats.
-constexpr int64_t kMaxCtas = 1024;
 
 int64_t partial_floats(int tile_heads, int pitch) {
   return int64_t{2} * tile_heads * pitch;
@@ -1066,17 +1105,26 @@ int64_t units_bound(int64_t batch, int64_t rows, int64_t max_len, int unit) {
   return per == 0 ? 0 : batch > INT64_MAX / 4096 / per ? INT64_MAX / 4096 : batch * per;
 }
 
-// Grid of the first kernel: one wave, no more CTAs than units.
-int64_t split_ctas(int64_t units, int64_t resident) {
-  return std::max<int64_t>(1, std::min({units, resident, kMaxCtas}));
+// Grid of the first kernel: one wave of `per_sm` CTAs an SM, no more than units.
+int64_t split_ctas(int64_t units, int per_sm) {
+  return std::max<int64_t>(1, std::min<int64_t>(units, int64_t{per_sm} * sm_count()));
 }
 
-template <typename T>
+// CTAs an SM at most: what the sums' registers leave, and what bounds the partials.
+constexpr int kMmaCtasPerSm = 4;
+constexpr int simt_ctas_per_sm(int heads) { return heads >= 4 ? 4 : 8; }
+
+template <typename T, int E>
 int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
   const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
   if (max_len <= int64_t{1} << sp.unit_log) return KPB_OK;  // no row has a second unit to share
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(c.sh.batch * sp.rows));
+  // warps per head: enough for 16 an SM where heads are few, one where they are many
+  const int64_t heads = c.sh.batch * c.sh.q_heads;
+  int share_log = 0;
+  while (2 << share_log <= kJoinWarps && (heads << (share_log + 1)) <= int64_t{16} * sm_count())
+    ++share_log;
+  cfg.gridDim = dim3(static_cast<unsigned>(cdiv(heads, kJoinWarps >> share_log)));
   cfg.blockDim = dim3(kJoinWarps * kWarp);
   cfg.stream = c.s;
   cudaLaunchAttribute attr[1];
@@ -1084,8 +1132,8 @@ int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  KPB_CUDA(cudaLaunchKernelEx(&cfg, join_rows<T>, c.seq_lens, static_cast<T*>(c.o), c.sh, sp, ctas,
-                              c.err));
+  KPB_CUDA(cudaLaunchKernelEx(&cfg, join_rows<T, E>, c.seq_lens, static_cast<T*>(c.o), c.sh, sp,
+                              ctas, share_log, c.err));
   return KPB_OK;
 }
 
@@ -1096,8 +1144,8 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, 
   sp.tiles = static_cast<int>(cdiv(sp.group, tile_heads));
   sp.rows = c.sh.lay.heads * sp.tiles;
   sp.pitch = pitch;
-  for (sp.unit_log = 0; 1 << sp.unit_log < unit; ++sp.unit_log) {
-  }
+  sp.unit_log = log2_of(unit);
+  sp.page_log = log2_of(c.sh.lay.page_size);
   sp.bases = static_cast<int64_t*>(ws);
   sp.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + bases_bytes(c.sh.batch));
   return sp;
@@ -1111,13 +1159,13 @@ int launch_simt(const PagedCall& c, void* ws) {
   if (int rc = occupancy_blocks(reinterpret_cast<const void*>(kernel), kSplitThreads, 0, &occ))
     return rc;
   const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, kSimtUnit);
-  const int64_t ctas = split_ctas(units, int64_t{occ} * sm_count());
+  const int64_t ctas = split_ctas(units, std::min(occ, simt_ctas_per_sm(HG)));
   kernel<<<static_cast<unsigned>(ctas), kSplitThreads, 0, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T>(c, sp, ctas);
+  return launch_join<T, E>(c, sp, ctas);
 }
 
 // Heads per tile: the smallest of 1, 2, 4, 8 that holds the group, 8 for larger ones.
@@ -1140,20 +1188,20 @@ int dispatch_simt(const PagedCall& c, void* ws) {
 template <typename T, typename C, int DP, int NT>
 int launch_mma(const PagedCall& c, void* ws) {
   using Plan = MmaPlan<C, DP, NT>;
-  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, Plan::kUnit, ws);
+  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, Plan::kKeys, ws);
   auto* kernel = split_mma<T, C, DP, NT>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   if (int rc = ensure_dyn_smem(fn, Plan::kSmem)) return rc;
   int occ = 0;
   if (int rc = occupancy_blocks(fn, kSplitThreads, Plan::kSmem, &occ)) return rc;
-  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, Plan::kUnit);
-  const int64_t ctas = split_ctas(units, int64_t{occ} * sm_count());
+  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, Plan::kKeys);
+  const int64_t ctas = split_ctas(units, std::min(occ, kMmaCtasPerSm));
   kernel<<<static_cast<unsigned>(ctas), kSplitThreads, Plan::kSmem, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T>(c, sp, ctas);
+  return launch_join<T, DP / kWarp>(c, sp, ctas);
 }
 
 // Sixteen heads to a tile where the group has more than eight, so that its keys are read
@@ -1201,13 +1249,15 @@ int launch(int variant, const PagedCall& c, void* ws) {
 size_t paged_attention_workspace_bytes(int variant, int64_t batch, int64_t q_heads,
                                        int64_t k_heads, int64_t dim, int64_t max_len) {
   if (variant == 0) return 0;
-  // the widest tile and pitch that any of the ways takes for this call, and as many CTAs as
-  // there can be units (a tile holds one head at least)
+  // the widest tile and pitch that either way takes for this call, and as many workers as
+  // there can be warps and units (a tile holds one head at least, a unit 16 keys); the
+  // CUDA-core way has twice the CTAs for tiles of a quarter of the heads
   const int pitch = static_cast<int>(dim <= 64 ? 64 : dim <= 128 ? 128 : 256) + 4;
   const int heads = q_heads / k_heads > 8 && dim <= 128 ? 16 : 8;
-  const int64_t ctas = split_ctas(units_bound(batch, q_heads, max_len, kSimtUnit), kMaxCtas);
+  const int64_t units = units_bound(batch, q_heads, max_len, kSimtUnit);
+  const int64_t workers = std::min(units, kSplitWarps * split_ctas(units, kMmaCtasPerSm));
   return bases_bytes(batch) +
-         static_cast<size_t>(ctas * partial_floats(heads, pitch)) * sizeof(float);
+         static_cast<size_t>(workers * partial_floats(heads, pitch)) * sizeof(float);
 }
 
 int paged_attention(int variant, int dtype, int cache_dtype, const void* q, const void* k_cache,
