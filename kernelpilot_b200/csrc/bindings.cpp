@@ -299,7 +299,9 @@ CacheArgs check_cache(const at::Tensor& kc, const at::Tensor& vc,
   CacheArgs a;
   a.pages = kc.size(0), a.heads = kc.size(1), a.page_size = kc.size(2), a.dim = kc.size(3);
   for (const at::Tensor* c : {&kc, &vc})
-    TORCH_CHECK(c->numel() == 0 || c->select(0, 0).is_contiguous(),
+    TORCH_CHECK(c->numel() == 0 || ((a.dim == 1 || c->stride(3) == 1) &&
+                                    (a.page_size == 1 || c->stride(2) == a.dim) &&
+                                    (a.heads == 1 || c->stride(1) == a.page_size * a.dim)),
                 "each page of a cache must be contiguous");
   TORCH_CHECK(a.pages < 2 || kc.stride(0) == vc.stride(0),
               "k_cache and v_cache must have the same page stride");

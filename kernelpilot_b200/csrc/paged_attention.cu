@@ -392,17 +392,27 @@ __device__ __forceinline__ int64_t key_row(const int* __restrict__ table, int64_
 // ------------------------------------------------------------------ variant 1: split_simt
 
 constexpr int kSimtUnit = 16;
+constexpr int kSimtKeys = 4;  // keys that a warp takes at a time
 
-// Lanes are strided over a row's elements (E each); a warp takes 4 keys at a time and HG
-// query heads: 4 * HG products, summed over the lanes by halving, so that each lane ends
-// with the score of one (key, head).
-template <typename T, typename C, int E, int HG>
+// Stages of the ring of 4 keys and values per thread: up to 64 KB a CTA.
+constexpr int simt_stages(int E) { return E == 8 ? 2 : E == 4 ? 3 : 4; }
+constexpr int simt_ring_bytes(int E) {
+  return simt_stages(E) * kSimtKeys * 2 * E * 4 * kSplitThreads;
+}
+constexpr int simt_vector(int E) { return E == 2 ? 2 : 4; }
+
+// A lane holds E of a row's elements; a warp takes 4 keys at a time and HG query heads:
+// 4 * HG products, summed over the lanes by halving, so that each lane ends with the score
+// of one (key, head). kRing (fp32 rows in whole vectors): elements in vectors of 8 or 16
+// bytes, each thread's own through its own slots of a shared-memory ring, groups of 4 keys
+// simt_stages - 1 ahead. Else: elements strided over the lanes, read where they are used.
+template <typename T, typename C, int E, int HG, bool kRing>
 __global__ void __launch_bounds__(kSplitThreads)
 split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __restrict__ v_cache,
            const int* __restrict__ table, const int* __restrict__ seq_lens,
            const float* __restrict__ k_scale, const float* __restrict__ v_scale,
            T* __restrict__ o, PagedShape sh, SplitShape sp, unsigned* err) {
-  constexpr int kKeys = 4;
+  constexpr int kKeys = kSimtKeys;
   constexpr int kSums = kKeys * HG;
   constexpr int kLog = kSums == 32 ? 5 : kSums == 16 ? 4 : kSums == 8 ? 3 : 2;
   constexpr int kSpread = 5 - kLog;  // 2^kSpread neighbouring lanes hold the same sum
@@ -415,6 +425,64 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
   int count;
   UnitPlace p = find_units(seq_lens, sh, sp, &scratch, &worker, &count, err);
   const int my_key = (lane >> kSpread) / HG;
+  constexpr int VE = kRing ? simt_vector(E) : 1, kVectors = E / VE, kS = simt_stages(E);
+  const auto element = [&](int e) { return (e / VE * kWarp + lane) * VE + e % VE; };
+
+  // the ring's loader: the unit, group of keys and rows (lane j: key j of the unit) that it
+  // loads next, and which of the units in flight hold a bad page
+  extern __shared__ __align__(16) float ring[];
+  UnitPlace lp = p;
+  int left = kRing ? count : 0, group = 0;
+  int64_t next_row = -1, unused = 0;
+  unsigned bad_units = 0, load_unit = 0, unit = 0;
+  const auto slot_of = [&](int stage, int key, int which, int v) {
+    return ((((stage * kKeys + key) * 2 + which) * kVectors + v) * kSplitThreads +
+            static_cast<int>(threadIdx.x)) * VE;
+  };
+  const auto look_up = [&]() {
+    next_row = -1;
+    if (left > 0 && lane < kSimtUnit)
+      next_row = key_row(table, lp.b, lp.blk * kSimtUnit + lane, lp.n,
+                         static_cast<uint32_t>(lp.row) / sp.tiles, sh, &unused, err);
+  };
+  const auto load = [&](int stage) {
+    if (left > 0) {
+      if (group == 0) {
+        const unsigned bit = 1u << (load_unit & 31);
+        bad_units = __any_sync(kFull, next_row == -2) ? bad_units | bit : bad_units & ~bit;
+      }
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) {
+        const int64_t row = __shfl_sync(kFull, next_row, group * kKeys + k);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+          const int i = element(v * VE);
+          const bool in = row >= 0 && i < dim;
+          const int64_t at = in ? row + i : 0;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const auto* src = reinterpret_cast<const char*>((w == 0 ? k_cache : v_cache) + at);
+            const uint32_t dst = smem_u32(ring + slot_of(stage, k, w, v));
+            if constexpr (VE == 4) cp_async16(dst, src, in);
+            else cp_async8(dst, src, in);
+          }
+        }
+      }
+      if (++group * kKeys >= min(kSimtUnit, lp.n - lp.blk * kSimtUnit)) {
+        group = 0;
+        ++load_unit;
+        if (--left > 0) lp.next(seq_lens, sh, sp, err);
+        look_up();
+      }
+    }
+    cp_async_commit();  // an empty group where nothing is left, so that the count stays
+  };
+  int stage = 0;
+  if constexpr (kRing) {
+    look_up();
+#pragma unroll
+    for (int i = 0; i < kS - 1; ++i) load(i);
+  }
 
   float qr[HG][E], acc[HG][E], m = -INFINITY, l = 0.f;
   bool fresh = true, whole_start = p.blk == 0;
@@ -428,7 +496,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
         const T* qh = q + p.b * sh.q_stride + (hk * sp.group + first + h) * dim;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int i = lane + e * kWarp;
+          const int i = element(e);
           qr[h][e] = i < dim && first + h < sp.group ? to_f(qh[i]) * (sh.scale * kLog2e) : 0.f;
           acc[h][e] = 0.f;
         }
@@ -439,10 +507,11 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
     }
     const int key0 = p.blk * kSimtUnit;
     int64_t my_scale = 0;
-    const int64_t my_row = lane < kSimtUnit
-                               ? key_row(table, p.b, key0 + lane, p.n, hk, sh, &my_scale, err)
-                               : -1;
-    if (__any_sync(kFull, my_row == -2)) l = nan_f();
+    int64_t my_row = -1;
+    if constexpr (!kRing) {
+      if (lane < kSimtUnit) my_row = key_row(table, p.b, key0 + lane, p.n, hk, sh, &my_scale, err);
+    }
+    if (kRing ? bad_units >> (unit++ & 31) & 1 : __any_sync(kFull, my_row == -2)) l = nan_f();
     float ks = 1.f, vs = 1.f;
     if constexpr (kQuant) {
       if (my_row >= 0) {
@@ -453,17 +522,32 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
 #pragma unroll 1
     for (int j = 0; j < kSimtUnit && key0 + j < p.n; j += kKeys) {
       float kv[kKeys][E], vv[kKeys][E];
-      int64_t row[kKeys];
+      if constexpr (kRing) {
+        load(stage == 0 ? kS - 1 : stage - 1);
+        cp_async_wait<kS - 1>();
 #pragma unroll
-      for (int k = 0; k < kKeys; ++k) row[k] = __shfl_sync(kFull, my_row, j + k);
+        for (int k = 0; k < kKeys; ++k) {
 #pragma unroll
-      for (int k = 0; k < kKeys; ++k) {
+          for (int v = 0; v < kVectors; ++v) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = lane + e * kWarp;
-          const bool in = i < dim && row[k] >= 0;
-          kv[k][e] = in ? cache_value(k_cache + row[k], i, 1.f) : 0.f;
-          vv[k][e] = in ? cache_value(v_cache + row[k], i, 1.f) : 0.f;
+            for (int e = 0; e < VE; ++e) {
+              kv[k][v * VE + e] = ring[slot_of(stage, k, 0, v) + e];
+              vv[k][v * VE + e] = ring[slot_of(stage, k, 1, v) + e];
+            }
+          }
+        }
+        stage = stage + 1 == kS ? 0 : stage + 1;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) {
+          const int64_t row = __shfl_sync(kFull, my_row, j + k);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int i = element(e);
+            const bool in = i < dim && row >= 0;
+            kv[k][e] = in ? cache_value(k_cache + row, i, 1.f) : 0.f;
+            vv[k][e] = in ? cache_value(v_cache + row, i, 1.f) : 0.f;
+          }
         }
       }
       float s[kSums];
@@ -493,8 +577,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       for (int off = (1 << kSpread) >> 1; off > 0; off >>= 1)
         score += __shfl_xor_sync(kFull, score, off);
       if constexpr (kQuant) score *= __shfl_sync(kFull, ks, j + my_key);
-      const int64_t key_at = __shfl_sync(kFull, my_row, j + my_key);  // below 0 past the end
-      if (key_at < 0) score = -INFINITY;
+      if (key0 + j + my_key >= p.n) score = -INFINITY;
       float top = score;
 #pragma unroll
       for (int off = HG << kSpread; off < kWarp; off <<= 1)
@@ -540,7 +623,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
         float* part = partial_at(sp, worker, slot, h);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int i = lane + e * kWarp;
+          const int i = element(e);
           if (!whole) part[i] = acc[h][e];
           else if (i < dim) out[i] = from_f<T>(acc[h][e] / hs);
         }
@@ -555,6 +638,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
     }
     p.next(seq_lens, sh, sp, err);
   }
+  if constexpr (kRing) cp_async_wait<0>();
   zero_empty(o, seq_lens, sh, err);
 }
 
@@ -1151,16 +1235,21 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, 
   return sp;
 }
 
-template <typename T, typename C, int E, int HG>
+template <typename T, typename C, int E, int HG, bool kRing>
 int launch_simt(const PagedCall& c, void* ws) {
   const SplitShape sp = split_shape(c, HG, E * kWarp + 4, kSimtUnit, ws);
-  auto* kernel = split_simt<T, C, E, HG>;
+  auto* kernel = split_simt<T, C, E, HG, kRing>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  constexpr int kSmem = kRing ? simt_ring_bytes(E) : 0;
+  if (kSmem > 0) {
+    if (int rc = ensure_dyn_smem(fn, kSmem)) return rc;
+  }
   int occ = 0;
-  if (int rc = occupancy_blocks(reinterpret_cast<const void*>(kernel), kSplitThreads, 0, &occ))
-    return rc;
-  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, kSimtUnit);
+  if (int rc = occupancy_blocks(fn, kSplitThreads, kSmem, &occ)) return rc;
+  const int64_t units =
+      units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, kSimtUnit);
   const int64_t ctas = split_ctas(units, std::min(occ, simt_ctas_per_sm(HG)));
-  kernel<<<static_cast<unsigned>(ctas), kSplitThreads, 0, c.s>>>(
+  kernel<<<static_cast<unsigned>(ctas), kSplitThreads, kSmem, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
@@ -1168,14 +1257,27 @@ int launch_simt(const PagedCall& c, void* ws) {
   return launch_join<T, E>(c, sp, ctas);
 }
 
+template <typename T, typename C, int E, int HG>
+int dispatch_simt_ring(const PagedCall& c, void* ws) {
+  if constexpr (std::is_same_v<C, float>) {
+    constexpr int VE = simt_vector(E);
+    const uintptr_t both =
+        reinterpret_cast<uintptr_t>(c.k_cache) | reinterpret_cast<uintptr_t>(c.v_cache);
+    if (c.sh.lay.dim % VE == 0 && both % (VE * 4) == 0 &&
+        (c.sh.lay.num_pages < 2 || c.sh.lay.page_stride % VE == 0))
+      return launch_simt<T, C, E, HG, true>(c, ws);
+  }
+  return launch_simt<T, C, E, HG, false>(c, ws);
+}
+
 // Heads per tile: the smallest of 1, 2, 4, 8 that holds the group, 8 for larger ones.
 template <typename T, typename C, int E>
 int dispatch_simt_heads(const PagedCall& c, void* ws) {
   const int64_t group = c.sh.q_heads / c.sh.lay.heads;
-  if (group <= 1) return launch_simt<T, C, E, 1>(c, ws);
-  if (group <= 2) return launch_simt<T, C, E, 2>(c, ws);
-  if (group <= 4) return launch_simt<T, C, E, 4>(c, ws);
-  return launch_simt<T, C, E, 8>(c, ws);
+  if (group <= 1) return dispatch_simt_ring<T, C, E, 1>(c, ws);
+  if (group <= 2) return dispatch_simt_ring<T, C, E, 2>(c, ws);
+  if (group <= 4) return dispatch_simt_ring<T, C, E, 4>(c, ws);
+  return dispatch_simt_ring<T, C, E, 8>(c, ws);
 }
 
 template <typename T, typename C>
