@@ -145,7 +145,7 @@ struct SplitShape {
   int pitch;
   int unit_log;      // log2 of the keys per unit
   int page_log;      // log2 of the page size, -1 where it is no power of two
-  int64_t* bases;    // workspace: units before each sequence (batch), then their total
+  int2* shared;      // workspace: [sequence][row], (first partial, partials) where workers share it
   float* partials;   // workspace: [worker][2][tile_heads][pitch]
 };
 
@@ -204,16 +204,15 @@ struct UnitPlace {
   }
 };
 
-// What find_units needs of shared memory.
+// What find_units needs of shared memory; total stays there.
 struct FindScratch {
-  int64_t warp_sum[kSplitWarps], upto[kSplitThreads];
+  int64_t warp_sum[kSplitWarps], upto[kSplitThreads], total;
 };
 
 // This warp's worker number, its count of units and the place of the first. Every thread
 // calls it: thread i adds up the units of the i-th run of sequences, a scan gives each run
 // its first unit, and each warp looks its own unit up among the runs. Workers are dealt out
-// over the CTAs first, so that few units spread over all SMs. CTA 0 leaves bases and total
-// in the workspace.
+// over the CTAs first, so that few units spread over all SMs.
 __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens,
                                                 const PagedShape& sh, const SplitShape& sp,
                                                 FindScratch* scratch, int64_t* worker, int* count,
@@ -239,14 +238,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
     total += scratch->warp_sum[w];
   }
   scratch->upto[threadIdx.x] = upto;
-  if (blockIdx.x == 0) {
-    int64_t base = upto - mine;
-    for (int64_t b = b0; b < b1; ++b) {
-      sp.bases[b] = base;
-      base += units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
-    }
-    if (threadIdx.x == 0) sp.bases[sh.batch] = total;
-  }
+  if (threadIdx.x == 0) scratch->total = total;
   __syncthreads();
   const int64_t workers = workers_of(gridDim.x, total);
   *worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
@@ -274,14 +266,17 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   return p;
 }
 
-// Zeros for the sequences without keys, strided over the CTAs.
+// Zeros for the sequences without keys, strided over the CTAs; no worker shares their rows.
 template <typename T>
 __device__ __forceinline__ void zero_empty(T* __restrict__ o, const int* __restrict__ seq_lens,
-                                           const PagedShape& sh, unsigned* err) {
+                                           const PagedShape& sh, const SplitShape& sp,
+                                           unsigned* err) {
   const int64_t row = sh.q_heads * sh.lay.dim;
   for (int64_t b = blockIdx.x; b < sh.batch; b += gridDim.x) {
     if (keys_of(seq_lens, b, sh, err) != 0) continue;
     for (int64_t i = threadIdx.x; i < row; i += kSplitThreads) o[b * row + i] = from_f<T>(0.f);
+    for (int64_t i = threadIdx.x; i < sp.rows; i += kSplitThreads)
+      sp.shared[b * sp.rows + i] = make_int2(0, 0);
   }
 }
 
@@ -292,56 +287,78 @@ __device__ __forceinline__ float* partial_at(const SplitShape& sp, int64_t worke
   return sp.partials + ((worker * 2 + slot) * sp.tile_heads + h) * sp.pitch;
 }
 
+// Says for the row of place p, whose first unit this worker had, which partials it is in:
+// none if it is `whole`, else this worker's `slot` and slot 0 of the workers after it up to
+// the one with the row's last unit. `left`: this worker's units from p on.
+__device__ __forceinline__ void note_shared(const UnitPlace& p, bool whole, int64_t worker,
+                                            int slot, int left, const FindScratch* scratch,
+                                            const SplitShape& sp) {
+  int2 note = make_int2(0, 0);
+  if (!whole) {
+    const Deal deal(scratch->total, workers_of(gridDim.x, scratch->total));
+    const int64_t last = deal.first(worker + 1) - left + (p.blocks - 1 - p.blk);
+    note = make_int2(static_cast<int>(worker * 2 + slot),
+                     static_cast<int>(deal.worker_of(last) - worker) + 1);
+  }
+  sp.shared[p.b * sp.rows + p.row] = note;
+}
+
 // The partials of a (sequence, query head) whose row several workers share, joined by
 // 2^share_log of a CTA's warps: each takes every so manieth partial, lanes strided over the
 // values, as out = sum_c f_c O_c / sum_c f_c l_c, f_c = 2^(m_c - max m) carried along as a
-// running maximum; then the warps in order. `ctas` is the first kernel's grid.
+// running maximum; then the warps in order.
 constexpr int kJoinWarps = 16;
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kJoinWarps * kWarp)
-join_rows(const int* __restrict__ seq_lens, T* __restrict__ o, PagedShape sh, SplitShape sp,
-          int64_t ctas, int share_log, unsigned* err) {
+join_rows(T* __restrict__ o, int heads, int dim, SplitShape sp, int share_log) {
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][E * kWarp];
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
+  constexpr int kAhead = E == 8 ? 4 : 8;
   const int share = 1 << share_log, part = warp & (share - 1), first_warp = warp - part;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kJoinWarps >> share_log) + (warp >> share_log);
-  const bool live = at < sh.batch * sh.q_heads;
-  const int64_t b = live ? div_fast(at, sh.q_heads) : 0;
-  const int head = live ? static_cast<int>(at - b * sh.q_heads) : 0;
-  const int64_t blocks = units_of(keys_of(seq_lens, b, sh, err), sp);
-  const int hk = head / sp.group, g = head - hk * sp.group;
+  // head `at` of all sequences' heads: group at / sp.group of all key heads
+  const int64_t head = static_cast<int64_t>(blockIdx.x) * (kJoinWarps >> share_log) +
+                       (warp >> share_log);
+  const int at = static_cast<int>(head);
+  const bool live = head < heads;
+  const int hk = live ? at / sp.group : 0, g = live ? at - hk * sp.group : 0;
   const int tile = g / sp.tile_heads;
   pdl_wait_primary();
-  const int64_t total = sp.bases[sh.batch], base = sp.bases[b];
-  int count = 0;
+  const int2 note = live ? sp.shared[static_cast<int64_t>(hk) * sp.tiles + tile] : make_int2(0, 0);
+  const int count = note.y;
   float m = -INFINITY, l = 0.f, acc[E] = {};
-  if (live && blocks > 1) {
-    const int64_t workers = workers_of(ctas, total);
-    const int64_t u0 = base + (static_cast<int64_t>(hk) * sp.tiles + tile) * blocks;
-    const Deal deal(total, workers);
-    const int64_t w0 = deal.worker_of(u0);
-    count = static_cast<int>(deal.worker_of(u0 + blocks - 1) - w0) + 1;
-    if (count > 1) {
-      // only the first worker's part may begin inside its units (slot 1)
-      const int h = g - tile * sp.tile_heads;
-      const float* p0 = partial_at(sp, w0, u0 > deal.first(w0) ? 1 : 0, h);
-      const float* rest = partial_at(sp, w0, 0, h);
-      const int64_t step = static_cast<int64_t>(2) * sp.tile_heads * sp.pitch;
-#pragma unroll 4
-      for (int c = part; c < count; c += share) {
+  if (count > 1) {
+    const int h = g - tile * sp.tile_heads;
+    const float* p0 = partial_at(sp, note.x >> 1, note.x & 1, h);
+    const float* rest = partial_at(sp, note.x >> 1, 0, h);
+    const int64_t step = static_cast<int64_t>(2) * sp.tile_heads * sp.pitch;
+    // kAhead partials are loaded before the first is used, the last few under a guard
+    for (int c0 = part; c0 < count; c0 += kAhead * share) {
+      float v[kAhead][E], pm[kAhead], pl[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int c = c0 + i * share;
         const float* p = c == 0 ? p0 : rest + c * step;
-        float v[E];
+        pm[i] = c < count ? p[E * kWarp] : -INFINITY;
+        pl[i] = c < count ? p[E * kWarp + 1] : 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = p[lane + e * kWarp];
-        const float pm = p[E * kWarp], pl = p[E * kWarp + 1];
-        const float top = fmaxf(m, pm), to = top == -INFINITY ? 0.f : top;
-        const float f = ex2f(m - to), pf = ex2f(pm - to);
-        l = fmaf(l, f, pl * pf);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], f, v[e] * pf);
-        m = top;
+        for (int e = 0; e < E; ++e) v[i][e] = c < count ? p[lane + e * kWarp] : 0.f;
       }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = fmaxf(top, pm[i]);
+      const float to = top == -INFINITY ? 0.f : top, f = ex2f(m - to);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float pf = ex2f(pm[i] - to);
+        l = fmaf(pl[i], pf, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(v[i][e], pf, acc[e]);
+      }
+      m = top;
     }
   }
   if (share > 1) {
@@ -363,8 +380,7 @@ join_rows(const int* __restrict__ seq_lens, T* __restrict__ o, PagedShape sh, Sp
     }
   }
   if (count < 2) return;
-  const int dim = static_cast<int>(sh.lay.dim);
-  T* out = o + (b * sh.q_heads + head) * dim;
+  T* out = o + head * dim;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int i = lane + e * kWarp;
@@ -614,6 +630,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
       for (int off = HG << kSpread; off < kWarp; off <<= 1)
         sum += __shfl_xor_sync(kFull, sum, off);
       const bool whole = whole_start && row_ends;
+      if (whole_start && lane == 0) note_shared(p, whole, worker, slot, count, &scratch, sp);
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
         const float hs = __shfl_sync(kFull, sum, h << kSpread);
@@ -639,7 +656,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
     p.next(seq_lens, sh, sp, err);
   }
   if constexpr (kRing) cp_async_wait<0>();
-  zero_empty(o, seq_lens, sh, err);
+  zero_empty(o, seq_lens, sh, sp, err);
 }
 
 // ------------------------------------------------------------------ variant 1: split_mma
@@ -1120,6 +1137,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     const bool row_ends = p.blk + 1 == p.blocks;
     if (row_ends || count == 1) {
       const bool whole = whole_start && row_ends;
+      if (whole_start && lane == 0) note_shared(p, whole, worker, slot, count, scratch, sp);
       const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
       const int first = static_cast<int>(p.row - hk * sp.tiles) * kHeads;
 #pragma unroll
@@ -1160,7 +1178,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     p.next(seq_lens, sh, sp, err);
   }
   cp_async_wait<0>();
-  zero_empty(o, seq_lens, sh, err);
+  zero_empty(o, seq_lens, sh, sp, err);
 }
 
 // ------------------------------------------------------------------ launch
@@ -1179,8 +1197,8 @@ int64_t partial_floats(int tile_heads, int pitch) {
   return int64_t{2} * tile_heads * pitch;
 }
 
-size_t bases_bytes(int64_t batch) {
-  return static_cast<size_t>(cdiv((batch + 1) * static_cast<int64_t>(sizeof(int64_t)), 16) * 16);
+size_t notes_bytes(int64_t rows) {
+  return static_cast<size_t>(cdiv(rows * static_cast<int64_t>(sizeof(int2)), 16) * 16);
 }
 
 // Units of a call if every sequence were as long as its table allows.
@@ -1199,12 +1217,12 @@ constexpr int kMmaCtasPerSm = 4;
 constexpr int simt_ctas_per_sm(int heads) { return heads >= 4 ? 4 : 8; }
 
 template <typename T, int E>
-int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
+int launch_join(const PagedCall& c, const SplitShape& sp) {
   const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
   if (max_len <= int64_t{1} << sp.unit_log) return KPB_OK;  // no row has a second unit to share
   cudaLaunchConfig_t cfg = {};
   // warps per head: enough for 16 an SM where heads are few, one where they are many
-  const int64_t heads = c.sh.batch * c.sh.q_heads;
+  const int64_t heads = c.sh.batch * c.sh.q_heads;  // below 2^31
   int share_log = 0;
   while (2 << share_log <= kJoinWarps && (heads << (share_log + 1)) <= int64_t{16} * sm_count())
     ++share_log;
@@ -1216,8 +1234,9 @@ int launch_join(const PagedCall& c, const SplitShape& sp, int64_t ctas) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  KPB_CUDA(cudaLaunchKernelEx(&cfg, join_rows<T, E>, c.seq_lens, static_cast<T*>(c.o), c.sh, sp,
-                              ctas, share_log, c.err));
+  KPB_CUDA(cudaLaunchKernelEx(&cfg, join_rows<T, E>, static_cast<T*>(c.o),
+                              static_cast<int>(heads), static_cast<int>(c.sh.lay.dim), sp,
+                              share_log));
   return KPB_OK;
 }
 
@@ -1230,8 +1249,9 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, 
   sp.pitch = pitch;
   sp.unit_log = log2_of(unit);
   sp.page_log = log2_of(c.sh.lay.page_size);
-  sp.bases = static_cast<int64_t*>(ws);
-  sp.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + bases_bytes(c.sh.batch));
+  sp.shared = static_cast<int2*>(ws);
+  sp.partials =
+      reinterpret_cast<float*>(static_cast<char*>(ws) + notes_bytes(c.sh.batch * sp.rows));
   return sp;
 }
 
@@ -1254,7 +1274,7 @@ int launch_simt(const PagedCall& c, void* ws) {
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T, E>(c, sp, ctas);
+  return launch_join<T, E>(c, sp);
 }
 
 template <typename T, typename C, int E, int HG>
@@ -1303,7 +1323,7 @@ int launch_mma(const PagedCall& c, void* ws) {
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T, DP / kWarp>(c, sp, ctas);
+  return launch_join<T, DP / kWarp>(c, sp);
 }
 
 // Sixteen heads to a tile where the group has more than eight, so that its keys are read
@@ -1358,7 +1378,7 @@ size_t paged_attention_workspace_bytes(int variant, int64_t batch, int64_t q_hea
   const int heads = q_heads / k_heads > 8 && dim <= 128 ? 16 : 8;
   const int64_t units = units_bound(batch, q_heads, max_len, kSimtUnit);
   const int64_t workers = std::min(units, kSplitWarps * split_ctas(units, kMmaCtasPerSm));
-  return bases_bytes(batch) +
+  return notes_bytes(batch * q_heads) +
          static_cast<size_t>(workers * partial_floats(heads, pitch)) * sizeof(float);
 }
 
