@@ -201,7 +201,7 @@ int kpb_qk_norm_rope_backward(int variant, int dtype, const void* grad_q, const 
  *
  * write: row (t, h) of k and v (heads of a token contiguous, tokens k_stride / v_stride
  * elements apart) to slot slots[t]; slots below 0 are skipped; nothing else of the caches
- * changes. E4M3: the scale is the smallest power of two (>= 2^-126) that brings the row's
+ * changes; the caches must not overlap k, v or one another. E4M3: the scale is the smallest power of two (>= 2^-126) that brings the row's
  * largest magnitude to at most 448 (1 for a row of zeros), and a code is x / scale rounded
  * to nearest even; a row holding an infinity or NaN gets the scale NaN and zero codes.
  * Slots of one call must differ: of two tokens with one slot, either's elements may stay.
@@ -225,10 +225,13 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * offset j % page_size of the cache above. q is (B, Hq, D) with sequences q_stride
  * elements apart, o contiguous; Hq a multiple of Hkv. seq_lens[b] = 0 gives zeros. Cache
  * rows past a sequence's last key and table entries past its last page are not read.
- * E4M3 scales must not be negative, and codes must not be NaN (a cache written by
- * kpb_kv_cache_write has neither).
+ * A score of NaN or +inf, or no score above -inf, makes the head's output NaN, as the
+ * softmax does; a page outside the cache makes the sequence's heads NaN, a length past the
+ * table is cut to it and a negative one is none (bit 2 either way).
+ * Value scales of an E4M3 cache must not be negative; those of one sequence may span 2^28
+ * before weights lose bits to the largest.
  * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size),
- * 16-byte aligned, the call's own until it has run. */
+ * asked for on the device of the call, 16-byte aligned, the call's own until it has run. */
 size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,
                                            int64_t D, int64_t max_len);
 int kpb_paged_attention(int variant, int dtype, int cache_dtype, const void* q,

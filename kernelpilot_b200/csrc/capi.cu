@@ -283,7 +283,7 @@ extern "C" {
 
 const char* kpb_last_error(void) { return g_last_error.c_str(); }
 
-int kpb_version(void) { return 100; }
+int kpb_version(void) { return 101; }
 
 int kpb_num_variants(const char* op) {
   if (op == nullptr) return -1;
@@ -532,6 +532,8 @@ int kpb_kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, c
   if (!k || !v || !slots) return fail(KPB_EINVAL, "kv_cache_write: null pointer");
   if (num_pages > 0 && k_cache == v_cache)
     return fail(KPB_EINVAL, "kv_cache_write: k_cache and v_cache must differ");
+  if (num_pages > 0 && cache_dtype == KPB_E4M3 && k_scale == v_scale)
+    return fail(KPB_EINVAL, "kv_cache_write: k_scale and v_scale must differ");
   if (off_by(k, elem_bytes(dtype)) || off_by(v, elem_bytes(dtype)) || off_by(slots, 8))
     return fail(KPB_EINVAL, "kv_cache_write: tensors must be element-aligned");
   unsigned* err = nullptr;

@@ -1352,7 +1352,7 @@ bool mma_takes(const PagedCall& c) {
 
 template <typename T, typename C>
 int launch(int variant, const PagedCall& c, void* ws) {
-  if (variant == 0) {
+  if (variant == 0 || c.sh.lay.num_pages == 0) {  // no page to point a copy at
     paged_cta_head<T, C><<<static_cast<unsigned>(c.sh.batch * c.sh.q_heads), 128, 0, c.s>>>(
         static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
         static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,

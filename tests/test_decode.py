@@ -182,7 +182,7 @@ def _rope_back(L, variant=1, dtype=2, T=4, D=64, rot=64, ws=P, ws_bytes=1 << 30,
 
 
 def _write(L, variant=1, dtype=2, cache=2, T=4, H=2, D=64, pages=3, page=16, stride=None,
-           kc=P, vc=ctypes.c_void_p(8192), ks=P, vs=P, k=P):
+           kc=P, vc=ctypes.c_void_p(8192), ks=P, vs=ctypes.c_void_p(8192), k=P):
     stride = H * page * D if stride is None else stride
     return L.kpb_kv_cache_write(variant, dtype, cache, k, P, P, kc, vc, ks, vs, T, H, D, pages,
                                 page, H * D, H * D, stride, None)
@@ -239,6 +239,7 @@ def _paged(L, variant=1, dtype=2, cache=2, B=2, Hq=4, H=2, D=64, pages=3, page=1
     (lambda L: _write(L, cache=3, vs=ODD), "aligned"),
     (lambda L: _write(L, kc=ODD), "aligned"),
     (lambda L: _write(L, vc=P), "differ"),
+    (lambda L: _write(L, cache=3, vs=P), "differ"),
     (lambda L: _read(L, variant=2), "variant"),
     (lambda L: _read(L, cache=0), "cache dtype"),
     (lambda L: _read(L, slots=None), "null"),

@@ -395,7 +395,8 @@ def test_paged_attention(shape, dtype, e4m3, variant):
 @pytest.mark.parametrize("variant", VARIANTS)
 @pytest.mark.parametrize("e4m3", [0, 1])
 @pytest.mark.parametrize("lens", [[0], [1], [0, 0, 0], [0, 5, 0, 200, 1, 0], [63, 64, 65, 128],
-                                  [15, 16, 17, 31, 33], [3000] + [1] * 40, [1] * 40 + [3000]],
+                                  [15, 16, 17, 31, 33], [3000] + [1] * 40, [1] * 40 + [3000],
+                                  [0] * 300 + [33, 1] + [0] * 300 + [90] * 100],
                          ids=lambda v: f"{len(v)}x{max(v)}")
 def test_paged_attention_of_ragged_and_empty_sequences(lens, e4m3, variant):
     for dtype in (torch.float32, torch.bfloat16):
@@ -747,6 +748,7 @@ def test_the_operators_refuse_what_they_do_not_take():
     refuse("Long", write, k, v, slots.int(), kc, vc, ks, vs, 1)
     refuse("scales must", write, k, v, slots, kc, vc, ks[:1], vs, 1)
     refuse("differ", write, k, v, slots, kc, kc, ks, vs, 1)
+    refuse("differ", write, k, v, slots, kc, vc, ks, ks, 1)
     refuse("must be contiguous", write, k, v, slots, kc.transpose(1, 2), vc.transpose(1, 2),
            ks, vs, 1)
     refuse("float32, float16 and bfloat16", read, kc, vc, slots, ks, vs, torch.float64, 1)
@@ -790,6 +792,17 @@ def test_empty_inputs(variant):
                                          variant) == 0)
     assert ops.paged_attention(q[:0], *caches[:2], none[:0], lens[:0], None, None, None,
                                variant).shape == (0, 4, 64)
+    # a cache without pages: every page of a sequence is outside it
+    device_errors()
+    pool = [c[:0] for c in caches[:2]]
+    lens[1] = 3
+    table = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    got = ops.paged_attention(q, *pool, table, lens, None, None, None, variant)
+    assert torch.all(got[0] == 0) and torch.isnan(got[1]).all() and device_errors() == 4
+    rows = ops.kv_cache_read(*pool, slots[:2], None, None, k.dtype, variant)
+    assert all(torch.isnan(r).all() for r in rows) and device_errors() == 4
+    ops.kv_cache_write(k[:2], v[:2], slots[:2], *pool, None, None, variant)
+    assert device_errors() == 4
 
 
 def test_registry_runs_the_operators():
