@@ -7,10 +7,17 @@
 //
 //   variant 0  one warp per (token, head), lanes strided over the row's elements
 //   variant 1  a row's 16-byte vectors (of the uncompressed side) over neighbouring lanes,
-//              key and value row of a (token, head) loaded together before either is used;
-//              one short-lived thread per vector pair, so the scheduler keeps every SM's
-//              loads in flight. Needs rows of whole vectors on vector boundaries; other
-//              layouts take variant 0.
+//              two to a lane; key and value row of a (token, head) loaded together before
+//              either is used; one short-lived thread per four vectors, so the scheduler
+//              keeps every SM's loads in flight. A row's largest magnitude is found on
+//              packed 16-bit patterns. Bound by HBM, the e4m3 write nearly as much by its
+//              instructions. Needs rows of whole vectors on vector boundaries; other layouts
+//              take variant 0.
+//
+// Measured on B200 (6464 GB/s copy), 8 heads of 128, pages of 16: e4m3 write of 32768 bf16
+// tokens 35 us (204 MB; 31.5 us at copy bandwidth), variant 0 125; bf16 read of 65536 tokens
+// 83 us (537 MB; 83), variant 0 163; e4m3 read of 5001 tokens 5.7 us (31 MB; 4.8). With one
+// vector a lane and unpacked maxima the write took 54 us, the reads 89 and 7.4.
 #include "kp_kv_cache.cuh"
 
 namespace kpb {

@@ -17,11 +17,25 @@
 //              (maximum, sum, weighted values), joined in order by a second kernel (a
 //              programmatic dependent). Each warp streams its own keys and values and no
 //              barrier stands in its way: with the four warps of a CTA on one row instead,
-//              meeting in shared memory at each row's end, every call took 8 us more. Two
-//              ways to the products:
+//              meeting in shared memory at each row's end, the calls below took 13.6 us for
+//              the one sequence and 113 for e4m3 (10.7 and 103 with warps at that step; the
+//              bf16 batch 173 and 175). Two ways to the products:
 //                split_mma   fp16 / bf16 q, rows a multiple of 16 bytes on 16-byte
 //                            boundaries: cp.async into a swizzled ring per warp, mma.sync
+//                            (a key head's 1 to 16 query heads fill 8-wide fragments; of a
+//                            128-row tcgen05 tile they would fill a few rows, and the
+//                            tensor pipe is 16 to 28% busy as it is)
 //                split_simt  everything else (fp32, odd head dims, odd bases)
+//
+// What bounds it: the keys' and values' bytes; for e4m3, with half the bytes a value, their
+// conversion to fp16 and the warps' latency as much. Measured on B200 (6464 GB/s copy), head
+// dim 128, 8 key heads, ragged lengths:
+//   64 sequences up to 8192 keys, bf16, 32 query heads    174 us (1065 MB; 165 at that rate)
+//   32 sequences up to 16384 keys, e4m3, 64 query heads   101 us (549 MB; 85)
+//   64 sequences up to 4096 keys, fp32, 32 query heads    194 us (1066 MB; 165)
+//   2 sequences up to 32768 keys, fp16, 32 heads of 64     76 us (434 MB; 67)
+//   one sequence of 1037 keys, bf16, 32 query heads       10.4 us, 3 of them the join's launch
+// variant 0 takes 4764, 9193, -, 12317 and 274 us on the same calls.
 #include <algorithm>
 
 #include "kp_kv_cache.cuh"

@@ -62,7 +62,9 @@ def generator(seed):
 
 ROPE_SHAPES = [(1, 1, 1, 2), (1, 32, 8, 128), (3, 5, 1, 7), (17, 4, 4, 64), (33, 6, 2, 80),
                (2, 64, 8, 128), (130, 3, 1, 256), (5, 2, 2, 33), (9, 7, 3, 96), (700, 32, 8, 128),
-               (11, 0, 3, 64), (6, 3, 0, 64), (40, 1, 1, 1), (2100, 4, 2, 64)]
+               (11, 0, 3, 64), (6, 3, 0, 64), (40, 1, 1, 1), (2100, 4, 2, 64),
+               # enough rows for several heads a turn and many turns, heads no multiple of four
+               (3001, 27, 3, 128), (1301, 30, 2, 80)]
 
 
 def rope_limits(q, k, wq, wk):
@@ -381,7 +383,8 @@ PAGED_SHAPES = [(1, 1, 1, 16, 1, 1), (1, 8, 2, 64, 100, 16), (3, 32, 8, 128, 257
                 (2, 20, 1, 128, 333, 100), (1, 32, 8, 128, 1037, 16), (7, 8, 8, 64, 900, 32),
                 (2, 24, 2, 96, 515, 48), (1, 4, 4, 128, 5000, 16), (130, 4, 2, 64, 90, 16),
                 (3, 9, 3, 8, 64, 3), (2, 40, 1, 64, 200, 128), (2, 4, 1, 256, 700, 16),
-                (1, 1, 1, 1, 65, 2), (2, 34, 2, 128, 400, 16), (1, 10, 10, 112, 150, 16)]
+                (1, 1, 1, 1, 65, 2), (2, 34, 2, 128, 400, 16), (1, 10, 10, 112, 150, 16),
+                (1, 8, 1, 128, 40000, 16)]
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
