@@ -201,10 +201,11 @@ int kpb_qk_norm_rope_backward(int variant, int dtype, const void* grad_q, const 
  *
  * write: row (t, h) of k and v (heads of a token contiguous, tokens k_stride / v_stride
  * elements apart) to slot slots[t]; slots below 0 are skipped; nothing else of the caches
- * changes; the caches must not overlap k, v or one another. E4M3: the scale is the smallest power of two (>= 2^-126) that brings the row's
- * largest magnitude to at most 448 (1 for a row of zeros), and a code is x / scale rounded
- * to nearest even; a row holding an infinity or NaN gets the scale NaN and zero codes.
- * Slots of one call must differ: of two tokens with one slot, either's elements may stay.
+ * changes; the caches must not overlap k, v or one another. E4M3: the scale is the smallest
+ * power of two (>= 2^-126) that brings the row's largest magnitude to at most 448 (1 for a
+ * row of zeros), and a code is x / scale rounded to nearest even; a row holding an infinity
+ * or NaN gets the scale NaN and zero codes. Slots of one call must differ: of two tokens
+ * with one slot, either's elements may stay.
  *
  * read: k and v (T, Hkv, D) contiguous in `dtype` from slots[t]; E4M3 rows as code * scale
  * rounded once; rows of slots below 0 are zeros. Any scales may be read, not only powers

@@ -216,8 +216,8 @@ RopeArgs check_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   RopeArgs a;
   a.dtype = dtype_of(q);
   a.T = q.size(0), a.Hq = q.size(1), a.Hkv = k.size(1), a.D = q.size(2);
-  TORCH_CHECK(k.size(0) == a.T && k.size(2) == a.D, "q and k must match in tokens and head dim, got ",
-              q.sizes(), " and ", k.sizes());
+  TORCH_CHECK(k.size(0) == a.T && k.size(2) == a.D,
+              "q and k must match in tokens and head dim, got ", q.sizes(), " and ", k.sizes());
   for (const at::Tensor* w : {&wq, &wk}) {
     check_same_device(*w, q, "weight");
     TORCH_CHECK(w->is_contiguous() && w->dim() == 1 && w->size(0) == a.D,

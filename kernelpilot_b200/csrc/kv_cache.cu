@@ -117,7 +117,8 @@ struct Codes {
 template <typename T>
 __device__ __forceinline__ uint32_t max_bits(const uint4& v) {
   if constexpr (sizeof(T) == 4) {
-    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu),
+               max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
   } else {
     return __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
                     __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
@@ -145,8 +146,10 @@ __device__ __forceinline__ typename Codes<Vec<T>::kN>::type pack_codes(const flo
     float g[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = f[4 * i + j] * inv;
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo =
+        __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi =
+        __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE, __NV_E4M3);
     w[i] = lo | hi << 16;
   }
   if constexpr (N == 8) return make_uint2(w[0], w[1]);
@@ -172,8 +175,8 @@ template <typename T, typename C, int V>
 __global__ void __launch_bounds__(kVecThreads)
 write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
                   const int64_t* __restrict__ slots, C* k_cache, C* v_cache, float* k_scale,
-                  float* v_scale, int rows, int log_lanes, int page_log, int64_t k_stride, int64_t v_stride,
-                  KvLayout lay, unsigned* err) {
+                  float* v_scale, int rows, int log_lanes, int page_log, int64_t k_stride,
+                  int64_t v_stride, KvLayout lay, unsigned* err) {
   constexpr int N = Vec<T>::kN;
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
   const int64_t group = (static_cast<int64_t>(blockIdx.x) * kVecThreads + threadIdx.x) >> log_lanes;
@@ -219,7 +222,8 @@ write_vector_rows(const T* __restrict__ k, const T* __restrict__ v,
         float f[N];
         unpack<T>(raw[w][i], f);
         typename Codes<N>::type codes = pack_codes<T>(f, inv);
-        if (inv == 0.f) codes = typename Codes<N>::type{};  // a row that is not finite: NaN * 0 is no code of 0
+        // a row that is not finite: its NaN * 0 would be no code of 0
+        if (inv == 0.f) codes = typename Codes<N>::type{};
         if (j < nv) reinterpret_cast<typename Codes<N>::type*>(y)[j] = codes;
       }
       if (lane == 0) (w == 0 ? k_scale : v_scale)[lay.scale(page, h, off)] = s;
@@ -369,9 +373,9 @@ int kv_cache_write(int variant, int dtype, int cache_dtype, const void* k, const
                    const int64_t* slots, void* k_cache, void* v_cache, float* k_scale,
                    float* v_scale, int64_t tokens, int64_t k_stride, int64_t v_stride,
                    const KvLayout& lay, unsigned* err, cudaStream_t s) {
-#define KPB_WRITE(T, C)                                                                      \
-  launch_write<T, C>(variant, k, v, slots, k_cache, v_cache, k_scale, v_scale, tokens, k_stride,      \
-                     v_stride, lay, err, s)
+#define KPB_WRITE(T, C)                                                                  \
+  launch_write<T, C>(variant, k, v, slots, k_cache, v_cache, k_scale, v_scale, tokens,   \
+                     k_stride, v_stride, lay, err, s)
   const bool q = cache_dtype == KPB_E4M3;
   switch (dtype) {
     case KPB_F32: return q ? KPB_WRITE(float, uint8_t) : KPB_WRITE(float, float);

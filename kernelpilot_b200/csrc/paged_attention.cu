@@ -989,161 +989,161 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     __syncwarp();
     const uint32_t kt = ring + stage * Plan::kStage, vt = kt + Plan::kTile;
     const int key0 = p.blk * kKeys;
-    {
-      // scores: block l / 8 of an ldmatrix is keys (l / 8) % 2 * 8 .., chunk + l / 16
-      const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
-      // two chains of sums where a single 16-key tile would leave one
-      constexpr int kChains = kTiles * NT > 1 ? 1 : 2;
-      float c[kTiles][NT][kChains][4] = {};
+    // scores: block l / 8 of an ldmatrix is keys (l / 8) % 2 * 8 .., chunk + l / 16
+    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
+    // two chains of sums where a single 16-key tile would leave one
+    constexpr int kChains = kTiles * NT > 1 ? 1 : 2;
+    float c[kTiles][NT][kChains][4] = {};
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        if constexpr (!kQuant) {
+    for (int j = 0; j < kTiles; ++j) {
+      if constexpr (!kQuant) {
 #pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-            uint32_t a[4];
-            ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, 2 * kk + kch), a);
+        for (int kk = 0; kk < kSteps; ++kk) {
+          uint32_t a[4];
+          ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, 2 * kk + kch), a);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<M>(c[j][nt][kk % kChains], a[0], a[1], a[2], a[3], qb[nt][kk][0],
+                        qb[nt][kk][1]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < kSteps; kk += 2) {
+          uint32_t w[4];
+          ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half(w[2 * i], &a0, &a2);
+            codes_to_half(w[2 * i + 1], &a1, &a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<M>(c[j][nt][kk % kChains], a[0], a[1], a[2], a[3], qb[nt][kk][0], qb[nt][kk][1]);
-          }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < kSteps; kk += 2) {
-            uint32_t w[4];
-            ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t a0, a1, a2, a3;
-              codes_to_half(w[2 * i], &a0, &a2);
-              codes_to_half(w[2 * i + 1], &a1, &a3);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816<M>(c[j][nt][i % kChains], a0, a1, a2, a3, qb[nt][kk + i][0], qb[nt][kk + i][1]);
-            }
+              mma16816<M>(c[j][nt][i % kChains], a0, a1, a2, a3, qb[nt][kk + i][0],
+                          qb[nt][kk + i][1]);
           }
         }
       }
-      float ks[kTiles][2], vs[kTiles][2], shrink = 1.f;
-      if constexpr (kQuant) {
-        const float* sc = reinterpret_cast<const float*>(
-            smem + (warp * kS + stage) * Plan::kStage + 2 * Plan::kTile);
-        // the exponent above the largest finite value scale (positive: ordered as integers);
-        // past the last key the scale's place holds 0
-        const uint32_t mine = __float_as_uint(sc[kKeys + (lane & (kKeys - 1))]);
-        const uint32_t top =
-            min((__reduce_max_sync(kFull, mine >= 0x7f800000u ? 0u : mine) >> 23) + 1, 253u);
-        if (top > vref) {  // the sums so far become relative to the new one
-          shrink = exp2f(static_cast<float>(static_cast<int>(vref) - static_cast<int>(top)));
-          vref = top;
-        }
-        const float down = __uint_as_float((254 - vref) << 23);
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ks[j][h] = sc[16 * j + 8 * h + r];
-            vs[j][h] = sc[kKeys + 16 * j + 8 * h + r] * down;
-          }
-        }
+    }
+    float ks[kTiles][2], vs[kTiles][2], shrink = 1.f;
+    if constexpr (kQuant) {
+      const float* sc = reinterpret_cast<const float*>(
+          smem + (warp * kS + stage) * Plan::kStage + 2 * Plan::kTile);
+      // the exponent above the largest finite value scale (positive: ordered as integers);
+      // past the last key the scale's place holds 0
+      const uint32_t mine = __float_as_uint(sc[kKeys + (lane & (kKeys - 1))]);
+      const uint32_t top =
+          min((__reduce_max_sync(kFull, mine >= 0x7f800000u ? 0u : mine) >> 23) + 1, 253u);
+      if (top > vref) {  // the sums so far become relative to the new one
+        shrink = exp2f(static_cast<float>(static_cast<int>(vref) - static_cast<int>(top)));
+        vref = top;
       }
-      const bool full = key0 + kKeys <= p.n;
-      uint32_t hi[kTiles][NT][2], lo[kTiles][NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float w[kTiles][2][2], alpha[2];  // [16 keys][key r, r + 8][head 2t, 2t + 1]
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float s = c[j][nt][0][2 * h + i];
-              if constexpr (kChains == 2) s += c[j][nt][1][2 * h + i];
-              s *= kQuant ? mult[nt][i] * ks[j][h] : mult[nt][i];
-              if (!full && key0 + 16 * j + 8 * h + r >= p.n) s = -INFINITY;
-              w[j][h][i] = s;
-              top = fmaxf(top, s);
-            }
-          }
-#pragma unroll
-          for (int off = 4; off < kWarp; off <<= 1)
-            top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-          const float m_new = fmaxf(m[nt][i], top);
-          const float base = m_new == -INFINITY ? 0.f : m_new;
-          alpha[i] = ex2f(m[nt][i] - base);
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
-              sum += w[j][h][i];
-              if constexpr (kQuant) w[j][h][i] *= vs[j][h];
-            }
-          }
-          l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
-          m[nt][i] = m_new;
-          if constexpr (kQuant) alpha[i] *= shrink;
-        }
-        if (__any_sync(kFull, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[nt][kk][i] *= alpha[i & 1];
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t rest;
-            hi[j][nt][h] = transpose8(split_weights<M, !kQuant>(w[j][h][0], w[j][h][1], &rest));
-            lo[j][nt][h] = transpose8(rest);
-          }
-        }
-      }
-      // values, transposed on the way: 16-bit blocks are (keys 0-7, elements 0-7), (0-7,
-      // 8-15), (8-15, 0-7), (8-15, 8-15); e4m3 blocks as for the keys, two neighbouring
-      // elements of a key to a 16-bit unit
+      const float down = __uint_as_float((254 - vref) << 23);
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
-        if constexpr (!kQuant) {
-          const int vrow = (lane & 7) + (lane >> 4) * 8 + 16 * j, vch = (lane >> 3) & 1;
 #pragma unroll
-          for (int kk = 0; kk < kSteps; ++kk) {
-            uint32_t a[4];
-            ldmatrix4<true>(vt + tile_at<kRow>(vrow, 2 * kk + vch), a);
+        for (int h = 0; h < 2; ++h) {
+          ks[j][h] = sc[16 * j + 8 * h + r];
+          vs[j][h] = sc[kKeys + 16 * j + 8 * h + r] * down;
+        }
+      }
+    }
+    const bool full = key0 + kKeys <= p.n;
+    uint32_t hi[kTiles][NT][2], lo[kTiles][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[kTiles][2][2], alpha[2];  // [16 keys][key r, r + 8][head 2t, 2t + 1]
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float s = c[j][nt][0][2 * h + i];
+            if constexpr (kChains == 2) s += c[j][nt][1][2 * h + i];
+            s *= kQuant ? mult[nt][i] * ks[j][h] : mult[nt][i];
+            if (!full && key0 + 16 * j + 8 * h + r >= p.n) s = -INFINITY;
+            w[j][h][i] = s;
+            top = fmaxf(top, s);
+          }
+        }
+#pragma unroll
+        for (int off = 4; off < kWarp; off <<= 1)
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+        const float m_new = fmaxf(m[nt][i], top);
+        const float base = m_new == -INFINITY ? 0.f : m_new;
+        alpha[i] = ex2f(m[nt][i] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
+            sum += w[j][h][i];
+            if constexpr (kQuant) w[j][h][i] *= vs[j][h];
+          }
+        }
+        l[nt][i] = fmaf(l[nt][i], alpha[i], sum);
+        m[nt][i] = m_new;
+        if constexpr (kQuant) alpha[i] *= shrink;
+      }
+      if (__any_sync(kFull, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][kk][i] *= alpha[i & 1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t rest;
+          hi[j][nt][h] = transpose8(split_weights<M, !kQuant>(w[j][h][0], w[j][h][1], &rest));
+          lo[j][nt][h] = transpose8(rest);
+        }
+      }
+    }
+    // values, transposed on the way: 16-bit blocks are (keys 0-7, elements 0-7), (0-7,
+    // 8-15), (8-15, 0-7), (8-15, 8-15); e4m3 blocks as for the keys, two neighbouring
+    // elements of a key to a 16-bit unit
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      if constexpr (!kQuant) {
+        const int vrow = (lane & 7) + (lane >> 4) * 8 + 16 * j, vch = (lane >> 3) & 1;
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) {
+          uint32_t a[4];
+          ldmatrix4<true>(vt + tile_at<kRow>(vrow, 2 * kk + vch), a);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], hi[j][nt][0], hi[j][nt][1]);
+            mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], lo[j][nt][0], lo[j][nt][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < kSteps; kk += 2) {
+          uint32_t w[4];
+          ldmatrix4<true>(vt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // bytes: key 2t (two elements), key 2t + 1 (two) -> element by element
+            uint32_t a0, a1, a2, a3;
+            codes_to_half(__byte_perm(w[2 * i], 0, 0x3120), &a0, &a1);
+            codes_to_half(__byte_perm(w[2 * i + 1], 0, 0x3120), &a2, &a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], hi[j][nt][0], hi[j][nt][1]);
-              mma16816<M>(acc[nt][kk], a[0], a[1], a[2], a[3], lo[j][nt][0], lo[j][nt][1]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < kSteps; kk += 2) {
-            uint32_t w[4];
-            ldmatrix4<true>(vt + tile_at<kRow>(krow + 16 * j, kk + kch), w);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              // bytes: key 2t (two elements), key 2t + 1 (two) -> element by element
-              uint32_t a0, a1, a2, a3;
-              codes_to_half(__byte_perm(w[2 * i], 0, 0x3120), &a0, &a1);
-              codes_to_half(__byte_perm(w[2 * i + 1], 0, 0x3120), &a2, &a3);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, hi[j][nt][0], hi[j][nt][1]);
-                mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, lo[j][nt][0], lo[j][nt][1]);
-              }
+              mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, hi[j][nt][0], hi[j][nt][1]);
+              mma16816<M>(acc[nt][kk + i], a0, a1, a2, a3, lo[j][nt][0], lo[j][nt][1]);
             }
           }
         }
       }
-      if (bad_slots >> stage & 1) {
+    }
+    if (bad_slots >> stage & 1) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = nan_f();
-      }
+      for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = nan_f();
     }
     __syncwarp();  // every lane has read this stage before it is filled again
     stage = stage + 1 == kS ? 0 : stage + 1;
@@ -1330,7 +1330,8 @@ int launch_mma(const PagedCall& c, void* ws) {
   if (int rc = ensure_dyn_smem(fn, Plan::kSmem)) return rc;
   int occ = 0;
   if (int rc = occupancy_blocks(fn, kSplitThreads, Plan::kSmem, &occ)) return rc;
-  const int64_t units = units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, Plan::kKeys);
+  const int64_t units =
+      units_bound(c.sh.batch, sp.rows, c.sh.max_pages * c.sh.lay.page_size, Plan::kKeys);
   const int64_t ctas = split_ctas(units, std::min(occ, kMmaCtasPerSm));
   kernel<<<static_cast<unsigned>(ctas), kSplitThreads, Plan::kSmem, c.s>>>(
       static_cast<const T*>(c.q), static_cast<const C*>(c.k_cache),
@@ -1357,10 +1358,13 @@ int dispatch_mma(const PagedCall& c, void* ws) {
 template <typename C>
 bool mma_takes(const PagedCall& c) {
   const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  return c.sh.lay.dim * sizeof(C) % 16 == 0 && c.sh.lay.dim % 8 == 0 &&
+  const KvLayout& lay = c.sh.lay;
+  const int64_t extent = (lay.num_pages < 2 ? 0 : (lay.num_pages - 1) * lay.page_stride) +
+                         lay.heads * lay.page_size * lay.dim;
+  return lay.dim * sizeof(C) % 16 == 0 && lay.dim % 8 == 0 &&
          (at(c.k_cache) | at(c.v_cache)) % 16 == 0 &&
-         (c.sh.lay.num_pages < 2 || c.sh.lay.page_stride * sizeof(C) % 16 == 0) &&
-         c.sh.lay.num_pages * c.sh.lay.page_stride * static_cast<int64_t>(sizeof(C)) / 16 < kBadRow &&
+         (lay.num_pages < 2 || lay.page_stride * sizeof(C) % 16 == 0) &&
+         static_cast<int64_t>(extent * sizeof(C) / 16) < kBadRow &&
          at(c.q) % 8 == 0 && (c.sh.batch < 2 || c.sh.q_stride % 4 == 0);
 }
 
@@ -1410,7 +1414,8 @@ int paged_attention(int variant, int dtype, int cache_dtype, const void* q, cons
     case KPB_F32:
       return e4m3 ? launch<float, uint8_t>(variant, c, ws) : launch<float, float>(variant, c, ws);
     case KPB_F16:
-      return e4m3 ? launch<__half, uint8_t>(variant, c, ws) : launch<__half, __half>(variant, c, ws);
+      return e4m3 ? launch<__half, uint8_t>(variant, c, ws)
+                  : launch<__half, __half>(variant, c, ws);
     default:
       return e4m3 ? launch<__nv_bfloat16, uint8_t>(variant, c, ws)
                   : launch<__nv_bfloat16, __nv_bfloat16>(variant, c, ws);

@@ -488,7 +488,8 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
                        int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
                        int q_ctas, int log_lanes, RopeShape sh, unsigned* err) {
   using R = RawOf<T, VE>;
-  extern __shared__ __align__(16) unsigned char ring[];  // [stage][head][x a, x b, g a, g b][thread]
+  // [stage][head][x a, x b, g a, g b][thread]
+  extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float sums[kVecThreads / kWarp][kMaxHeadDim];
   pdl_launch_dependents();
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
@@ -539,7 +540,8 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
                            g + i * dim + pl.b};
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const uint32_t dst = smem_u32(ring) + slot(stage, i, v) * static_cast<uint32_t>(sizeof(R));
+          const uint32_t dst =
+              smem_u32(ring) + slot(stage, i, v) * static_cast<uint32_t>(sizeof(R));
           if constexpr (sizeof(R) == 16) cp_async16(dst, src[v], true);
           else cp_async8(dst, src[v], true);
         }
@@ -877,10 +879,11 @@ int qk_norm_rope(int variant, int dtype, const void* q, const void* k, const voi
                  int64_t rot, int64_t max_pos, int64_t q_stride, int64_t k_stride, float eps,
                  bool interleaved, unsigned* err, cudaStream_t s) {
   const RopeShape sh{tokens, q_heads, k_heads, dim, rot, max_pos, eps, interleaved};
-#define KPB_ROPE(T)                                                                       \
-  launch<T>(variant, static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(wq), \
-            static_cast<const T*>(wk), cos_sin, positions, static_cast<T*>(q_out),        \
-            static_cast<T*>(k_out), q_stride, k_stride, sh, err, s)
+#define KPB_ROPE(T)                                                                \
+  launch<T>(variant, static_cast<const T*>(q), static_cast<const T*>(k),          \
+            static_cast<const T*>(wq), static_cast<const T*>(wk), cos_sin,        \
+            positions, static_cast<T*>(q_out), static_cast<T*>(k_out), q_stride,  \
+            k_stride, sh, err, s)
   switch (dtype) {
     case KPB_F32: return KPB_ROPE(float);
     case KPB_F16: return KPB_ROPE(__half);

@@ -113,14 +113,16 @@ def test_cache_references_round_trip(e4m3):
         assert torch.all(y[3] == 0)
         live = slots >= 0
         if e4m3:  # three fraction bits: half a step is 2^-4 of the value, or of the smallest normal
-            step = torch.maximum(x[live].double().abs(), x[live].double().abs().amax(-1, True) / 2 ** 14)
+            mag = x[live].double().abs()
+            step = torch.maximum(mag, mag.amax(-1, True) / 2 ** 14)
             assert torch.all((y[live] - x[live].double()).abs() <= step * 2.0 ** -4)
         else:
             assert torch.equal(y[live], x[live].double())
     untouched = torch.ones(kc.shape[0] * kc.shape[2], dtype=torch.bool)
     untouched[slots[slots >= 0]] = False
     rest = untouched.nonzero()[:, 0]
-    assert torch.equal(kc[rest // 4, :, rest % 4].float(), caches[0][rest // 4, :, rest % 4].float())
+    assert torch.equal(kc[rest // 4, :, rest % 4].float(),
+                       caches[0][rest // 4, :, rest % 4].float())
 
 
 @pytest.mark.parametrize("e4m3", [0, 1])
