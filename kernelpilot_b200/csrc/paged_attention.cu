@@ -20,12 +20,12 @@
 //              meeting in shared memory at each row's end, the calls below took 13.6 us for
 //              the one sequence and 113 for e4m3 (10.7 and 103 with warps at that step; the
 //              bf16 batch 173 and 175). Two ways to the products:
-//                split_mma   fp16 / bf16 q, rows a multiple of 16 bytes on 16-byte
-//                            boundaries: cp.async into a swizzled ring per warp, mma.sync
+//                split_mma   fp16 / bf16 q, or fp32 q on an e4m3 cache up to D = 128, rows
+//                            a multiple of 16 bytes on 16-byte boundaries: cp.async into a swizzled ring per warp, mma.sync
 //                            (a key head's 1 to 16 query heads fill 8-wide fragments; of a
 //                            128-row tcgen05 tile they would fill a few rows, and the
 //                            tensor pipe is 16 to 28% busy as it is)
-//                split_simt  everything else (fp32, odd head dims, odd bases)
+//                split_simt  everything else (fp32 caches, odd head dims, odd bases)
 //
 // What bounds it: the keys' and values' bytes; for e4m3, with half the bytes a value, their
 // conversion to fp16 and the warps' latency as much. Measured on B200 (6464 GB/s copy), head
@@ -806,8 +806,9 @@ constexpr uint32_t kBadRow = 0xfffffffeu;  // in a page outside the cache
 // weights' fragments over (movmatrix) and adds O^T += V^T P^T (elements x heads). The
 // weights enter as two 16-bit parts (split_weights), so that they carry 2^-15 of themselves
 // (bf16) or 2^-21 (fp16); the second product is a small part of the time that loading takes.
-// e4m3: codes become fp16 in registers, q is scaled by a power of two to [1, 2) (exact) and
-// the key's scale multiplies its score. The value's scale multiplies the weight, relative to
+// e4m3: codes become fp16 in registers, q is scaled by a power of two to [1, 2) (exact; fp32
+// queries as two fp16 parts, 2^-22 of the largest element and less) and the key's scale
+// multiplies its score. The value's scale multiplies the weight, relative to
 // the power of two above the largest scale that the warp has met (the running sums follow
 // when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's full
 // fraction while its scale is above 2^-28 of the largest.
@@ -909,7 +910,8 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
 #pragma unroll
   for (int i = 0; i < kS - 1; ++i) load(i);
 
-  uint32_t qb[NT][kSteps][2];
+  constexpr int kParts = std::is_same_v<T, float> ? 2 : 1;  // 16-bit parts of q
+  uint32_t qb[kParts][NT][kSteps][2];
   float mult[NT][2];                      // score -> log2 units, heads 2t and 2t + 1
   float acc[NT][kSteps][4];               // O^T: elements x heads
   float m[NT][2], l[NT][2];               // running maximum and sum
@@ -932,27 +934,25 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int d = kk * 16 + i * 8 + 2 * t;
-              qb[nt][kk][i] =
+              qb[0][nt][kk][i] =
                   live && d < dim ? *reinterpret_cast<const uint32_t*>(qh + d) : 0u;
             }
           }
           mult[nt][0] = mult[nt][1] = sh.scale * kLog2e;
         } else {
           // elements 4t .. 4t+3 of each 16, in the order that a word of codes has them
+          using Raw = std::conditional_t<std::is_same_v<T, float>, float4, uint2>;
+          Raw raw[kSteps];
           uint32_t top = 0;
 #pragma unroll
           for (int kk = 0; kk < kSteps; ++kk) {
             const int d = kk * 16 + 4 * t;
-            uint2 raw = make_uint2(0u, 0u);
-            if (live && d < dim) raw = *reinterpret_cast<const uint2*>(qh + d);
-            qb[nt][kk][0] = raw.x;
-            qb[nt][kk][1] = raw.y;
+            raw[kk] = Raw{};
+            if (live && d < dim) raw[kk] = *reinterpret_cast<const Raw*>(qh + d);
+            const T* e = reinterpret_cast<const T*>(&raw[kk]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const T* e = reinterpret_cast<const T*>(&qb[nt][kk][i]);
-              top = max(top, __float_as_uint(to_f(e[0])) & 0x7fffffffu);
-              top = max(top, __float_as_uint(to_f(e[1])) & 0x7fffffffu);
-            }
+            for (int i = 0; i < 4; ++i)
+              top = max(top, __float_as_uint(to_f(e[i])) & 0x7fffffffu);
           }
           top = max(top, __shfl_xor_sync(kFull, top, 1));
           top = max(top, __shfl_xor_sync(kFull, top, 2));
@@ -962,11 +962,17 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           const float down = __uint_as_float((254 - ex) << 23), up = __uint_as_float(ex << 23);
 #pragma unroll
           for (int kk = 0; kk < kSteps; ++kk) {
+            const T* e = reinterpret_cast<const T*>(&raw[kk]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const T* e = reinterpret_cast<const T*>(&qb[nt][kk][i]);
-              const __half2 v = __floats2half2_rn(to_f(e[0]) * down, to_f(e[1]) * down);
-              qb[nt][kk][i] = *reinterpret_cast<const uint32_t*>(&v);
+              float x = to_f(e[2 * i]) * down, y = to_f(e[2 * i + 1]) * down;
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) {
+                const __half2 v = __floats2half2_rn(x, y);
+                qb[part][nt][kk][i] = *reinterpret_cast<const uint32_t*>(&v);
+                x -= __low2float(v);
+                y -= __high2float(v);
+              }
             }
           }
           // `up` of heads 2t and 2t + 1 lies with the lanes of rows 2t and 2t + 1
@@ -1003,8 +1009,8 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           ldmatrix4<false>(kt + tile_at<kRow>(krow + 16 * j, 2 * kk + kch), a);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma16816<M>(c[j][nt][kk % kChains], a[0], a[1], a[2], a[3], qb[nt][kk][0],
-                        qb[nt][kk][1]);
+            mma16816<M>(c[j][nt][kk % kChains], a[0], a[1], a[2], a[3], qb[0][nt][kk][0],
+                        qb[0][nt][kk][1]);
         }
       } else {
 #pragma unroll
@@ -1017,9 +1023,12 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
             codes_to_half(w[2 * i], &a0, &a2);
             codes_to_half(w[2 * i + 1], &a1, &a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816<M>(c[j][nt][i % kChains], a0, a1, a2, a3, qb[nt][kk + i][0],
-                          qb[nt][kk + i][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+                mma16816<M>(c[j][nt][i % kChains], a0, a1, a2, a3, qb[part][nt][kk + i][0],
+                            qb[part][nt][kk + i][1]);
+            }
           }
         }
       }
@@ -1341,10 +1350,8 @@ int launch_mma(const PagedCall& c, void* ws) {
   return launch_join<T, DP / kWarp>(c, sp);
 }
 
-// Sixteen heads to a tile where the group has more than eight, so that its keys are read
-// once; at D > 128 their sums would not fit the registers.
 template <typename T, typename C>
-int dispatch_mma(const PagedCall& c, void* ws) {
+int dispatch_mma_16(const PagedCall& c, void* ws) {
   const bool wide = c.sh.q_heads / c.sh.lay.heads > 8;
   if (c.sh.lay.dim <= 64)
     return wide ? launch_mma<T, C, 64, 2>(c, ws) : launch_mma<T, C, 64, 1>(c, ws);
@@ -1353,9 +1360,20 @@ int dispatch_mma(const PagedCall& c, void* ws) {
   return launch_mma<T, C, 256, 1>(c, ws);
 }
 
-// Rows of the cache whole 16-byte chunks on 16-byte boundaries (cp.async), q's rows on
-// 8-byte ones; the cache's 16-byte units counted in 32 bits (64 GB, of 180 on the card).
-template <typename C>
+// Sixteen heads to a tile where the group has more than eight, so that its keys are read
+// once; at D > 128, and with the two parts of fp32 queries, they would not fit the registers.
+template <typename T, typename C>
+int dispatch_mma(const PagedCall& c, void* ws) {
+  if constexpr (std::is_same_v<T, float>) {
+    return c.sh.lay.dim <= 64 ? launch_mma<T, C, 64, 1>(c, ws) : launch_mma<T, C, 128, 1>(c, ws);
+  } else {
+    return dispatch_mma_16<T, C>(c, ws);
+  }
+}
+
+// Rows of the cache whole 16-byte chunks on 16-byte boundaries (cp.async), four elements of q
+// on theirs; the cache's 16-byte units counted in 32 bits (64 GB, of 180 on the card).
+template <typename T, typename C>
 bool mma_takes(const PagedCall& c) {
   const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   const KvLayout& lay = c.sh.lay;
@@ -1365,7 +1383,7 @@ bool mma_takes(const PagedCall& c) {
          (at(c.k_cache) | at(c.v_cache)) % 16 == 0 &&
          (lay.num_pages < 2 || lay.page_stride * sizeof(C) % 16 == 0) &&
          static_cast<int64_t>(extent * sizeof(C) / 16) < kBadRow &&
-         at(c.q) % 8 == 0 && (c.sh.batch < 2 || c.sh.q_stride % 4 == 0);
+         at(c.q) % (4 * sizeof(T)) == 0 && (c.sh.batch < 2 || c.sh.q_stride % 4 == 0);
 }
 
 template <typename T, typename C>
@@ -1378,8 +1396,10 @@ int launch(int variant, const PagedCall& c, void* ws) {
     KPB_LAUNCHED("paged_attention variant 0");
     return KPB_OK;
   }
-  if constexpr (sizeof(T) == 2) {
-    if (mma_takes<C>(c)) return dispatch_mma<T, C>(c, ws);
+  // fp32 keys and values have no product that keeps their bits; e4m3 codes are exact in fp16
+  if constexpr (sizeof(T) == 2 || sizeof(C) == 1) {
+    if (mma_takes<T, C>(c) && (sizeof(T) == 2 || c.sh.lay.dim <= 128))
+      return dispatch_mma<T, C>(c, ws);
   }
   return dispatch_simt<T, C>(c, ws);
 }
