@@ -158,6 +158,7 @@ struct SplitShape {
   int tile_heads;
   int pitch;
   int unit_log;      // log2 of the keys per unit
+  int deal_log;      // log2 of the keys dealt out at a time: a unit, or a whole short row
   int page_log;      // log2 of the page size, -1 where it is no power of two
   int2* shared;      // workspace: [sequence][row], (first partial, partials) where workers share it
   float* partials;   // workspace: [worker][2][tile_heads][pitch]
@@ -189,13 +190,20 @@ struct Deal {
   }
 };
 
+// Shares that a row of n keys is dealt out in.
+__device__ __forceinline__ int shares_of(int64_t n, const SplitShape& sp) {
+  return static_cast<int>((n + (1 << sp.deal_log) - 1) >> sp.deal_log);
+}
+
 // Workers of a grid: its warps, but two units to a worker at least once there are 64 workers
 // (the second unit's loads run beside the first's; a worker less is a partial less to join).
-// Never more workers than units, so that every worker of a shared row has a part of it.
+// Never more workers than shares, so that every worker of a shared row has a part of it.
 constexpr int kMinUnits = 2;
 
-__device__ __forceinline__ int64_t workers_of(int64_t ctas, int64_t total) {
-  return min(ctas * kSplitWarps, max(total / kMinUnits, min(total, int64_t{64})));
+__device__ __forceinline__ int64_t workers_of(int64_t ctas, int64_t total, const SplitShape& sp) {
+  const int64_t most =
+      sp.deal_log > sp.unit_log ? total : max(total / kMinUnits, min(total, int64_t{64}));
+  return min(ctas * kSplitWarps, most);
 }
 
 // A place in the list of units: sequence, row, block of keys.
@@ -236,7 +244,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   const int64_t b0 = min(sh.batch, threadIdx.x * per), b1 = min(sh.batch, b0 + per);
   int64_t mine = 0;
   for (int64_t b = b0; b < b1; ++b)
-    mine += units_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
+    mine += shares_of(keys_of(seq_lens, b, sh, err), sp) * sp.rows;
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < kWarp; o <<= 1) {
@@ -254,7 +262,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   scratch->upto[threadIdx.x] = upto;
   if (threadIdx.x == 0) scratch->total = total;
   __syncthreads();
-  const int64_t workers = workers_of(gridDim.x, total);
+  const int64_t workers = workers_of(gridDim.x, total, sp);
   *worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
   UnitPlace p = {};
   *count = 0;
@@ -268,15 +276,28 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   for (int i = 0; i < kSplitThreads / kWarp; ++i)
     before += __popc(__ballot_sync(kFull, scratch->upto[i * kWarp + lane] <= begin));
   int64_t base = before == 0 ? 0 : scratch->upto[before - 1];
+  int shares;
   for (p.b = before * per;; ++p.b) {
     p.n = static_cast<int>(keys_of(seq_lens, p.b, sh, err));
-    p.blocks = units_of(p.n, sp);
-    const int64_t units = p.blocks * sp.rows;
-    if (begin < base + units) break;
-    base += units;
+    shares = shares_of(p.n, sp);
+    if (begin < base + shares * sp.rows) break;
+    base += shares * sp.rows;
   }
-  p.row = div_fast(begin - base, p.blocks);
-  p.blk = static_cast<int>(begin - base - p.row * p.blocks);
+  p.blocks = units_of(p.n, sp);
+  p.row = div_fast(begin - base, shares);
+  p.blk = static_cast<int>(begin - base - p.row * shares);  // 0 where whole rows are dealt out
+  if (sp.deal_log > sp.unit_log) {  // the units of the worker's rows, sequence by sequence
+    int left = *count, units = 0;
+    int64_t row = p.row;
+    for (int64_t b = p.b; left > 0; ++b, row = 0) {
+      const int blocks = units_of(keys_of(seq_lens, b, sh, err), sp);
+      if (blocks == 0) continue;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(left), sp.rows - row));
+      units += rows * blocks;
+      left -= rows;
+    }
+    *count = units;
+  }
   return p;
 }
 
@@ -309,7 +330,7 @@ __device__ __forceinline__ void note_shared(const UnitPlace& p, bool whole, int6
                                             const SplitShape& sp) {
   int2 note = make_int2(0, 0);
   if (!whole) {
-    const Deal deal(scratch->total, workers_of(gridDim.x, scratch->total));
+    const Deal deal(scratch->total, workers_of(gridDim.x, scratch->total, sp));
     const int64_t last = deal.first(worker + 1) - left + (p.blocks - 1 - p.blk);
     note = make_int2(static_cast<int>(worker * 2 + slot),
                      static_cast<int>(deal.worker_of(last) - worker) + 1);
@@ -1242,7 +1263,7 @@ constexpr int simt_ctas_per_sm(int heads) { return heads >= 4 ? 4 : 8; }
 template <typename T, int E>
 int launch_join(const PagedCall& c, const SplitShape& sp) {
   const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
-  if (max_len <= int64_t{1} << sp.unit_log) return KPB_OK;  // no row has a second unit to share
+  if (max_len <= int64_t{1} << sp.deal_log) return KPB_OK;  // no row is dealt out in parts
   cudaLaunchConfig_t cfg = {};
   // warps per head: enough for 16 an SM where heads are few, one where they are many
   const int64_t heads = c.sh.batch * c.sh.q_heads;  // below 2^31
@@ -1263,7 +1284,9 @@ int launch_join(const PagedCall& c, const SplitShape& sp) {
   return KPB_OK;
 }
 
-SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, void* ws) {
+// Rows of a table of up to `whole` keys are not dealt out in parts.
+SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, int whole,
+                       void* ws) {
   SplitShape sp;
   sp.group = static_cast<int>(c.sh.q_heads / c.sh.lay.heads);
   sp.tile_heads = tile_heads;
@@ -1271,6 +1294,8 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, 
   sp.rows = c.sh.lay.heads * sp.tiles;
   sp.pitch = pitch;
   sp.unit_log = log2_of(unit);
+  const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
+  sp.deal_log = max_len <= whole ? log2_of(whole) : sp.unit_log;
   sp.page_log = log2_of(c.sh.lay.page_size);
   sp.shared = static_cast<int2*>(ws);
   sp.partials =
@@ -1280,7 +1305,7 @@ SplitShape split_shape(const PagedCall& c, int tile_heads, int pitch, int unit, 
 
 template <typename T, typename C, int E, int HG, bool kRing>
 int launch_simt(const PagedCall& c, void* ws) {
-  const SplitShape sp = split_shape(c, HG, E * kWarp + 4, kSimtUnit, ws);
+  const SplitShape sp = split_shape(c, HG, E * kWarp + 4, kSimtUnit, kSimtUnit, ws);
   auto* kernel = split_simt<T, C, E, HG, kRing>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   constexpr int kSmem = kRing ? simt_ring_bytes(E) : 0;
@@ -1330,10 +1355,16 @@ int dispatch_simt(const PagedCall& c, void* ws) {
   return dispatch_simt_heads<T, C, 8>(c, ws);
 }
 
+// Where no sequence can have more than 64 keys a warp takes whole rows: their two to four
+// units take it less time than a second kernel takes to join them (one sequence of 32 keys
+// 6.4 us and not 8.0, of 64 the same; 64 sequences 7.0 and not 9.5, 8.8 and not 11.2). On
+// the CUDA cores a unit takes longer (one sequence of 64 fp32 keys 15.3 us and not 9.7).
+constexpr int kWholeRow = 64;
+
 template <typename T, typename C, int DP, int NT>
 int launch_mma(const PagedCall& c, void* ws) {
   using Plan = MmaPlan<C, DP, NT>;
-  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, Plan::kKeys, ws);
+  const SplitShape sp = split_shape(c, Plan::kHeads, Plan::kPitch, Plan::kKeys, kWholeRow, ws);
   auto* kernel = split_mma<T, C, DP, NT>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   if (int rc = ensure_dyn_smem(fn, Plan::kSmem)) return rc;

@@ -316,7 +316,7 @@ __device__ __forceinline__ float2 group_sum2(float2 v, int lanes) {
 // kRing: one wave of CTAs, a group's turns `step` apart, each thread's own vectors through
 // its own slots of a shared-memory ring (cp.async, kForwardStages - 1 turns ahead). Else one
 // turn to a group, its vectors read into registers.
-constexpr int kForwardStages = 2;
+constexpr int kForwardStages = 2;  // `stage ^ 1` below is the other one
 
 template <typename T, int VE, int HPG, bool kAdjacent, bool kRing>
 __global__ void __launch_bounds__(kRopeThreads, kRing ? 5 : 4)

@@ -399,7 +399,8 @@ def test_paged_attention(shape, dtype, e4m3, variant):
 @pytest.mark.parametrize("e4m3", [0, 1])
 @pytest.mark.parametrize("lens", [[0], [1], [0, 0, 0], [0, 5, 0, 200, 1, 0], [63, 64, 65, 128],
                                   [15, 16, 17, 31, 33], [3000] + [1] * 40, [1] * 40 + [3000],
-                                  [0] * 300 + [33, 1] + [0] * 300 + [90] * 100],
+                                  [0] * 300 + [33, 1] + [0] * 300 + [90] * 100,
+                                  [5, 64, 0, 33] * 400],
                          ids=lambda v: f"{len(v)}x{max(v)}")
 def test_paged_attention_of_ragged_and_empty_sequences(lens, e4m3, variant):
     for dtype in (torch.float32, torch.bfloat16):
