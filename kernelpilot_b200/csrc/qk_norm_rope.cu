@@ -475,7 +475,7 @@ rope_vector_pairs(const T* __restrict__ q, const T* __restrict__ k, const T* __r
 // (cp.async, kBackStages - 1 turns ahead), which takes no registers and no barrier: held in
 // registers, loads and sums together left 12 warps an SM. Partial weight gradients to
 // partials[cta][dim]: lanes that hold the same elements are added within a warp by halving,
-// then the warps in order.
+// then the warps in order. Without partials, one CTA to a weight writes its gradient itself.
 constexpr int kBackStages = 2;
 
 template <typename T, int VE, int HPG, bool kAdjacent>
@@ -484,9 +484,10 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
                        const T* __restrict__ q, const T* __restrict__ k,
                        const T* __restrict__ wq, const T* __restrict__ wk,
                        const float* __restrict__ cos_sin, const int64_t* __restrict__ positions,
-                       T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ partials,
-                       int64_t gq_stride, int64_t gk_stride, int64_t q_stride, int64_t k_stride,
-                       int q_ctas, int log_lanes, RopeShape sh, unsigned* err) {
+                       T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dwq,
+                       T* __restrict__ dwk, float* __restrict__ partials, int64_t gq_stride,
+                       int64_t gk_stride, int64_t q_stride, int64_t k_stride, int q_ctas,
+                       int log_lanes, RopeShape sh, unsigned* err) {
   using R = RawOf<T, VE>;
   // [stage][head][x a, x b, g a, g b][thread]
   extern __shared__ __align__(16) unsigned char ring[];
@@ -652,7 +653,12 @@ rope_back_vector_pairs(const T* __restrict__ gq, const T* __restrict__ gk,
     float total = 0.f;
 #pragma unroll
     for (int j = 0; j < kVecThreads / kWarp; ++j) total += sums[j][i];
-    partials[static_cast<int64_t>(blockIdx.x) * dim + i] = total;
+    if (partials != nullptr) {
+      partials[static_cast<int64_t>(blockIdx.x) * dim + i] = total;
+    } else {  // the only CTA of its weight; alone, the other has no rows
+      (is_q ? dwq : dwk)[i] = from_f<T>(total);
+      if (gridDim.x == 1) (is_q ? dwk : dwq)[i] = from_f<T>(0.f);
+    }
   }
 }
 
@@ -816,18 +822,22 @@ int launch_back_pairs(const T* gq, const T* gk, const T* q, const T* k, const T*
   // one wave, shared out by the heads; no more CTAs than there is work for, nor than partials
   const int64_t wave = int64_t{occ} * sm_count(), most = back_ctas(sh, sm_count());
   const int64_t heads = sh.q_heads + sh.k_heads;
+  // two turns of one CTA take less time than a second kernel
+  const auto threads_of = [&](int64_t h) { return sh.tokens * cdiv(h, HPG) << log; };
+  const bool alone = std::max(threads_of(sh.q_heads), threads_of(sh.k_heads)) <= 2 * kVecThreads;
   const auto ctas_of = [&](int64_t h) {
     if (h == 0 || sh.tokens == 0) return int64_t{0};
-    const int64_t items = sh.tokens * cdiv(h, HPG);
+    if (alone) return int64_t{1};
     return std::max<int64_t>(
-        1, std::min({cdiv(items << log, kVecThreads), wave * h / heads, most}));
+        1, std::min({cdiv(threads_of(h), kVecThreads), wave * h / heads, most}));
   };
   const int64_t nq = ctas_of(sh.q_heads), nk = ctas_of(sh.k_heads);
   if (nq + nk > 0) {
     kernel<<<static_cast<unsigned>(nq + nk), kVecThreads, kSmem, s>>>(
-        gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, partials, gq_stride, gk_stride,
-        q_stride, k_stride, static_cast<int>(nq), log, sh, err);
+        gq, gk, q, k, wq, wk, cos_sin, positions, dq, dk, dwq, dwk, alone ? nullptr : partials,
+        gq_stride, gk_stride, q_stride, k_stride, static_cast<int>(nq), log, sh, err);
     KPB_LAUNCHED("qk_norm_rope_backward vector pairs");
+    if (alone) return KPB_OK;
   }
   return finish_weights<T>({partials, nq, dim}, {partials + nq * dim, nk, dim}, dim, dwq, dwk,
                            nq + nk > 0, s);
