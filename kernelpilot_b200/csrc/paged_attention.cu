@@ -21,10 +21,11 @@
 //              the one sequence and 113 for e4m3 (10.7 and 103 with warps at that step; the
 //              bf16 batch 173 and 175). Two ways to the products:
 //                split_mma   fp16 / bf16 q, or fp32 q on an e4m3 cache up to D = 128, rows
-//                            a multiple of 16 bytes on 16-byte boundaries: cp.async into a swizzled ring per warp, mma.sync
-//                            (a key head's 1 to 16 query heads fill 8-wide fragments; of a
-//                            128-row tcgen05 tile they would fill a few rows, and the
-//                            tensor pipe is 16 to 28% busy as it is)
+//                            a multiple of 16 bytes on 16-byte boundaries: cp.async
+//                            into a swizzled ring per warp, mma.sync (a key head's
+//                            1 to 16 query heads fill 8-wide fragments; of a 128-row
+//                            tcgen05 tile they would fill a few rows, and the tensor
+//                            pipe is 16 to 28% busy as it is)
 //                split_simt  everything else (fp32 caches, odd head dims, odd bases)
 //
 // What bounds it: the keys' and values' bytes; for e4m3, with half the bytes a value, their
@@ -32,7 +33,7 @@
 // dim 128, 8 key heads, ragged lengths:
 //   64 sequences up to 8192 keys, bf16, 32 query heads    174 us (1065 MB; 165 at that rate)
 //   32 sequences up to 16384 keys, e4m3, 64 query heads   101 us (549 MB; 85)
-//   64 sequences up to 4096 keys, fp32, 32 query heads    194 us (1066 MB; 165)
+//   64 sequences up to 4096 keys, fp32, 32 query heads    184 us (1066 MB; 165)
 //   2 sequences up to 32768 keys, fp16, 32 heads of 64     76 us (434 MB; 67)
 //   one sequence of 1037 keys, bf16, 32 query heads       10.4 us, 3 of them the join's launch
 // variant 0 takes 4764, 9193, -, 12317 and 274 us on the same calls.
@@ -206,7 +207,9 @@ __device__ __forceinline__ int64_t workers_of(int64_t ctas, int64_t total, const
   return min(ctas * kSplitWarps, most);
 }
 
-// A place in the list of units: sequence, row, block of keys.
+// A place in the list of units: sequence, row, block of keys. The lengths are read several
+// times over; should another stream change them under a call, its results mean nothing, but
+// every loop here still ends at the last sequence and no partial past the workspace is read.
 struct UnitPlace {
   int64_t b, row;
   int blk, blocks;  // block within the row, blocks of the row
@@ -276,12 +279,16 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   for (int i = 0; i < kSplitThreads / kWarp; ++i)
     before += __popc(__ballot_sync(kFull, scratch->upto[i * kWarp + lane] <= begin));
   int64_t base = before == 0 ? 0 : scratch->upto[before - 1];
-  int shares;
-  for (p.b = before * per;; ++p.b) {
+  int shares = 0;
+  for (p.b = before * per; p.b < sh.batch; ++p.b) {
     p.n = static_cast<int>(keys_of(seq_lens, p.b, sh, err));
     shares = shares_of(p.n, sp);
     if (begin < base + shares * sp.rows) break;
     base += shares * sp.rows;
+  }
+  if (p.b >= sh.batch) {  // only where the lengths change under the call
+    *count = 0;
+    return p;
   }
   p.blocks = units_of(p.n, sp);
   p.row = div_fast(begin - base, shares);
@@ -289,7 +296,7 @@ __device__ __forceinline__ UnitPlace find_units(const int* __restrict__ seq_lens
   if (sp.deal_log > sp.unit_log) {  // the units of the worker's rows, sequence by sequence
     int left = *count, units = 0;
     int64_t row = p.row;
-    for (int64_t b = p.b; left > 0; ++b, row = 0) {
+    for (int64_t b = p.b; left > 0 && b < sh.batch; ++b, row = 0) {
       const int blocks = units_of(keys_of(seq_lens, b, sh, err), sp);
       if (blocks == 0) continue;
       const int rows = static_cast<int>(min(static_cast<int64_t>(left), sp.rows - row));
@@ -330,10 +337,11 @@ __device__ __forceinline__ void note_shared(const UnitPlace& p, bool whole, int6
                                             const SplitShape& sp) {
   int2 note = make_int2(0, 0);
   if (!whole) {
-    const Deal deal(scratch->total, workers_of(gridDim.x, scratch->total, sp));
+    const int64_t workers = workers_of(gridDim.x, scratch->total, sp);
+    const Deal deal(scratch->total, workers);
     const int64_t last = deal.first(worker + 1) - left + (p.blocks - 1 - p.blk);
     note = make_int2(static_cast<int>(worker * 2 + slot),
-                     static_cast<int>(deal.worker_of(last) - worker) + 1);
+                     static_cast<int>(min(deal.worker_of(last), workers - 1) - worker) + 1);
   }
   sp.shared[p.b * sp.rows + p.row] = note;
 }
@@ -346,7 +354,7 @@ constexpr int kJoinWarps = 16;
 
 template <typename T, int E>
 __global__ void __launch_bounds__(kJoinWarps * kWarp)
-join_rows(T* __restrict__ o, int heads, int dim, SplitShape sp, int share_log) {
+join_rows(T* __restrict__ o, int heads, int dim, SplitShape sp, int workers, int share_log) {
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][E * kWarp];
   const int lane = threadIdx.x & (kWarp - 1), warp = threadIdx.x / kWarp;
   constexpr int kAhead = E == 8 ? 4 : 8;
@@ -360,7 +368,8 @@ join_rows(T* __restrict__ o, int heads, int dim, SplitShape sp, int share_log) {
   const int tile = g / sp.tile_heads;
   pdl_wait_primary();
   const int2 note = live ? sp.shared[static_cast<int64_t>(hk) * sp.tiles + tile] : make_int2(0, 0);
-  const int count = note.y;
+  const bool sound = note.x >= 0 && note.y >= 0 && (note.x >> 1) + note.y <= workers;
+  const int count = sound ? note.y : 0;
   float m = -INFINITY, l = 0.f, acc[E] = {};
   if (count > 1) {
     const int h = g - tile * sp.tile_heads;
@@ -523,6 +532,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
         group = 0;
         ++load_unit;
         if (--left > 0) lp.next(seq_lens, sh, sp, err);
+        if (lp.b >= sh.batch) left = 0;
         look_up();
       }
     }
@@ -538,7 +548,7 @@ split_simt(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __re
   float qr[HG][E], acc[HG][E], m = -INFINITY, l = 0.f;
   bool fresh = true, whole_start = p.blk == 0;
   int slot = 0;
-  for (; count > 0; --count) {
+  for (; count > 0 && p.b < sh.batch; --count) {
     const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
     const int first = static_cast<int>(p.row - hk * sp.tiles) * HG;
     if (fresh) {
@@ -923,6 +933,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
         }
       }
       if (--left > 0) lp.next(seq_lens, sh, sp, err);
+      if (lp.b >= sh.batch) left = 0;
     }
     cp_async_commit();  // an empty group where nothing is left, so that the count stays
     look_up();
@@ -939,7 +950,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
   uint32_t vref = 1;                      // e4m3: exponent that value scales are relative to
   bool fresh = true, whole_start = p.blk == 0;
   int slot = 0, stage = 0;
-  for (; count > 0; --count) {
+  for (; count > 0 && p.b < sh.batch; --count) {
     if (fresh) {
       fresh = false;
       const int64_t hk = static_cast<uint32_t>(p.row) / sp.tiles;
@@ -1261,7 +1272,7 @@ constexpr int kMmaCtasPerSm = 4;
 constexpr int simt_ctas_per_sm(int heads) { return heads >= 4 ? 4 : 8; }
 
 template <typename T, int E>
-int launch_join(const PagedCall& c, const SplitShape& sp) {
+int launch_join(const PagedCall& c, const SplitShape& sp, int64_t workers) {
   const int64_t max_len = c.sh.max_pages * c.sh.lay.page_size;
   if (max_len <= int64_t{1} << sp.deal_log) return KPB_OK;  // no row is dealt out in parts
   cudaLaunchConfig_t cfg = {};
@@ -1280,7 +1291,7 @@ int launch_join(const PagedCall& c, const SplitShape& sp) {
   cfg.numAttrs = 1;
   KPB_CUDA(cudaLaunchKernelEx(&cfg, join_rows<T, E>, static_cast<T*>(c.o),
                               static_cast<int>(heads), static_cast<int>(c.sh.lay.dim), sp,
-                              share_log));
+                              static_cast<int>(workers), share_log));
   return KPB_OK;
 }
 
@@ -1322,7 +1333,7 @@ int launch_simt(const PagedCall& c, void* ws) {
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T, E>(c, sp);
+  return launch_join<T, E>(c, sp, std::min(units, ctas * kSplitWarps));
 }
 
 template <typename T, typename C, int E, int HG>
@@ -1378,7 +1389,7 @@ int launch_mma(const PagedCall& c, void* ws) {
       static_cast<const C*>(c.v_cache), c.table, c.seq_lens, c.k_scale, c.v_scale,
       static_cast<T*>(c.o), c.sh, sp, c.err);
   KPB_LAUNCHED("paged_attention split");
-  return launch_join<T, DP / kWarp>(c, sp);
+  return launch_join<T, DP / kWarp>(c, sp, std::min(units, ctas * kSplitWarps));
 }
 
 template <typename T, typename C>
