@@ -45,6 +45,15 @@ inline int log2_of(int64_t n) {
   return log;
 }
 
+// Whether a note on a row's partials in paged_attention's workspace, (worker * 2 + slot of the
+// first, how many), stays within the `workers` that there are. A note that no worker wrote
+// (lengths that changed under the call) holds whatever the workspace held, so any pair of
+// integers comes here; nothing is added that could pass 32 bits.
+__host__ __device__ constexpr bool note_is_sound(int first_slot, int count, int workers) {
+  return first_slot >= 0 && count >= 0 && first_slot >> 1 < workers &&
+         count <= workers - (first_slot >> 1);
+}
+
 __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 
 // Scale of an e4m3 row whose largest magnitude has the bit pattern `amax` (sign cleared;

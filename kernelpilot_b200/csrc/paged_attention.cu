@@ -368,8 +368,7 @@ join_rows(T* __restrict__ o, int heads, int dim, SplitShape sp, int workers, int
   const int tile = g / sp.tile_heads;
   pdl_wait_primary();
   const int2 note = live ? sp.shared[static_cast<int64_t>(hk) * sp.tiles + tile] : make_int2(0, 0);
-  const bool sound = note.x >= 0 && note.y >= 0 && (note.x >> 1) + note.y <= workers;
-  const int count = sound ? note.y : 0;
+  const int count = note_is_sound(note.x, note.y, workers) ? note.y : 0;
   float m = -INFINITY, l = 0.f, acc[E] = {};
   if (count > 1) {
     const int h = g - tile * sp.tile_heads;
