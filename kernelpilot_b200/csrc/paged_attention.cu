@@ -741,13 +741,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
+// The smallest fp16 number.
+constexpr float kHalfTiny = 0x1p-24f;
+
 // Weights w >= 0 as a pair of M (x in the low half), and as *rest what that leaves. Where
 // the values may hold infinities (kCut: not e4m3 codes) the pair is cut towards zero and the
-// rest is never 0 beside a weight that is not: an infinite value times the two is then an
-// infinity, not infinity * 0 or the difference of two.
+// rest is never 0 beside a weight that is not (fp16: that kHalfTiny is not above): an infinite
+// value times the two is then an infinity, not infinity * 0 or the difference of two.
 template <typename M, bool kCut>
 __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* rest) {
-  constexpr float kTiny = 1.f / (1 << 24);
   uint32_t hi;
   float2 f;
   if constexpr (std::is_same_v<M, __half>) {
@@ -760,8 +762,8 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
   }
   float rx = x - f.x, ry = y - f.y;
   if constexpr (kCut) {
-    rx = fmaxf(rx, fminf(x, kTiny));
-    ry = fmaxf(ry, fminf(y, kTiny));
+    rx = fmaxf(rx, fminf(x, kHalfTiny));
+    ry = fmaxf(ry, fminf(y, kHalfTiny));
   }
   if constexpr (std::is_same_v<M, __half>) {
     const __half2 v = __floats2half2_rn(rx, ry);
@@ -776,6 +778,18 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
 // Weights are held times 2^14 (the maximum's weight is 16384): fp16 then keeps its full
 // fraction down to 2^-28 of the largest weight and something down to 2^-38.
 constexpr float kWeightBits = 14.f;
+
+// Whether a tile of `bytes` bytes of fp16 holds an infinity (same answer in every lane).
+__device__ __forceinline__ bool tile_has_inf(const unsigned char* tile, int bytes) {
+  __half2 top = __half2half2(__ushort_as_half(0));  // NaNs stay out of the maximum
+  for (int i = (threadIdx.x & (kWarp - 1)) * 16; i < bytes; i += kWarp * 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + i);
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(h[e]));
+  }
+  return __any_sync(kFull, __hisinf(__low2half(top)) != 0 || __hisinf(__high2half(top)) != 0);
+}
 
 // Four e4m3 codes as two pairs of fp16, exactly.
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* lo, uint32_t* hi) {
@@ -1132,6 +1146,32 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
         for (int kk = 0; kk < kSteps; ++kk) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[nt][kk][i] *= alpha[i & 1];
+        }
+      }
+      // fp16: a weight below kHalfTiny (26 nats below the largest and more) is cut to 0, which
+      // is wrong beside an infinite value only: the tile is searched where there are any, and
+      // such weights raised to kHalfTiny beside one
+      if constexpr (!kQuant && std::is_same_v<M, __half>) {
+        uint32_t least = 0xffffffffu;  // bits - 1 of the smallest weight above 0
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) least = min(least, __float_as_uint(w[j][h][i]) - 1u);
+          }
+        }
+        if (__any_sync(kFull, least < __float_as_uint(kHalfTiny) - 1u) &&
+            tile_has_inf(smem + (warp * kS + stage) * Plan::kStage + Plan::kTile, Plan::kTile)) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                w[j][h][i] = w[j][h][i] > 0.f ? fmaxf(w[j][h][i], kHalfTiny) : w[j][h][i];
+            }
+          }
         }
       }
 #pragma unroll

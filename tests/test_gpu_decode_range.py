@@ -1,0 +1,67 @@
+"""The decode step's attention at the ends of its range, every variant against the float64
+reference."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import test_gpu_decode as base
+from kernelpilot_b200 import specs_decode as sd
+from kernelpilot_b200.specs import randn
+
+pytestmark = pytest.mark.gpu
+
+DEV = base.DEV
+VARIANTS = base.VARIANTS
+
+
+def rows_of(B, Hq, Hkv, D, n, dtype, seed):
+    """q, and keys and values in fp32 as (B, Hkv, n, D)."""
+    g = base.generator(seed)
+    q = randn((B, Hq, D), dtype, DEV, g)
+    k, v = (randn((B, Hkv, n, D), torch.float32, DEV, g) for _ in range(2))
+    return q, k, v
+
+
+def cache_of(rows, page, dtype, e4m3):
+    """(B, Hkv, n, D) rows into pages of their own: (cache, scales or None, table)."""
+    B, H, n, D = rows.shape
+    per = -(-n // page)
+    pool = torch.zeros(B, H, per * page, D, device=DEV)
+    pool[:, :, :n] = rows
+    pool = pool.view(B, H, per, page, D).transpose(1, 2).reshape(B * per, H, page, D)
+    table = torch.arange(B * per, dtype=torch.int32, device=DEV).view(B, per)
+    if not e4m3:
+        return pool.to(dtype), None, table
+    codes, scale = sd.e4m3_rows(pool)
+    return codes, scale.float(), table
+
+
+def inputs(q, k, v, dtype, e4m3, page=16):
+    kc, ks, table = cache_of(k, page, dtype, e4m3)
+    vc, vs, _ = cache_of(v, page, dtype, e4m3)
+    lens = torch.full((q.shape[0],), k.shape[2], dtype=torch.int32, device=DEV)
+    return q, kc, vc, table, lens, ks, vs
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", base.DTYPES)
+@pytest.mark.parametrize("gap", [15, 30, 45, 60])
+@pytest.mark.parametrize("n,best,at", [(40, 3, 20), (40, 20, 3), (300, 3, 250), (300, 250, 3)])
+def test_infinite_values_under_small_weights(n, best, at, gap, dtype, variant):
+    # every key but `best` is `gap` nats below it; two elements of key `at` are infinite. The
+    # weight is e^-gap, not zero, so the outputs are the infinities
+    for D in (64, 128):
+        q, k, v = rows_of(2, 4, 1, D, n, dtype, 1)
+        q.zero_()[..., 0] = 1.0
+        k[..., 0] = -float(gap)
+        k[:, :, best, 0] = 0.0
+        clean = inputs(q, k, v, dtype, 0)
+        v[:, :, at, 9], v[:, :, at, 5] = float("inf"), float("-inf")
+        ins = inputs(q, k, v, dtype, 0)
+        got = base.run_paged(ins, variant, 1.0)
+        (want,) = sd.paged_attention_reference(*ins, 1.0)
+        assert torch.all(got[..., 9] == float("inf")) and torch.all(got[..., 5] == float("-inf"))
+        live = torch.tensor([i for i in range(D) if i not in (5, 9)], device=DEV)
+        base.check(got[..., live], want[..., live], base.attention_limit(*clean, 1.0))
