@@ -230,7 +230,7 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * softmax does; a page outside the cache makes the sequence's heads NaN, a length past the
  * table is cut to it and a negative one is none (bit 2 either way).
  * Value scales of an E4M3 cache must not be negative; those of one sequence may span 2^28
- * before weights lose bits to the largest.
+ * before weights lose bits to the largest. Rows of zeros do not count, whatever their scale.
  * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size),
  * asked for on the device of the call, 16-byte aligned, the call's own until it has run. */
 size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,

@@ -820,6 +820,17 @@ __device__ __forceinline__ uint32_t tile_turn(int row0, int lr, int ch) {
   return row0 * kRow + (mine ^ static_cast<uint32_t>(kRow >= 128 ? (row0 & 7) << 4 : 0));
 }
 
+// Whether row `row` of a tile of e4m3 codes is all zeros (of either sign).
+template <int kRow>
+__device__ __forceinline__ bool row_is_zero(const unsigned char* tile, int row) {
+#pragma unroll 1
+  for (int ch = 0; ch < kRow / 16; ++ch) {
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + tile_at<kRow>(row, ch));
+    if (((v.x | v.y | v.z | v.w) & 0x7f7f7f7fu) != 0) return false;
+  }
+  return true;
+}
+
 // Shared memory of one CTA: kStages x (keys, values, scales) per warp. A warp takes 32 keys
 // at a time where a row is 128 bytes at most, else 16. As many stages as let three CTAs
 // share an SM, two at least and four at most; where two do not fit, two CTAs or one.
@@ -853,8 +864,8 @@ constexpr uint32_t kBadRow = 0xfffffffeu;  // in a page outside the cache
 // e4m3: codes become fp16 in registers, q is scaled by a power of two to [1, 2) (exact; fp32
 // queries as two fp16 parts, 2^-22 of the largest element and less) and the key's scale
 // multiplies its score. The value's scale multiplies the weight, relative to
-// the power of two above the largest scale that the warp has met (the running sums follow
-// when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's full
+// the power of two above the largest scale that the warp has met, rows of zeros aside (the
+// running sums follow when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's full
 // fraction while its scale is above 2^-28 of the largest.
 template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(kSplitThreads)
@@ -1080,16 +1091,24 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
     }
     float ks[kTiles][2], vs[kTiles][2], shrink = 1.f;
     if constexpr (kQuant) {
-      const float* sc = reinterpret_cast<const float*>(
+      float* sc = reinterpret_cast<float*>(
           smem + (warp * kS + stage) * Plan::kStage + 2 * Plan::kTile);
       // the exponent above the largest finite value scale (positive: ordered as integers);
       // past the last key the scale's place holds 0
-      const uint32_t mine = __float_as_uint(sc[kKeys + (lane & (kKeys - 1))]);
-      const uint32_t top =
-          min((__reduce_max_sync(kFull, mine >= 0x7f800000u ? 0u : mine) >> 23) + 1, 253u);
-      if (top > vref) {  // the sums so far become relative to the new one
-        shrink = exp2f(static_cast<float>(static_cast<int>(vref) - static_cast<int>(top)));
-        vref = top;
+      const auto above = [](uint32_t bits) { return min((bits >> 23) + 1, 253u); };
+      const int my_key = lane & (kKeys - 1);
+      uint32_t mine = __float_as_uint(sc[kKeys + my_key]);
+      if (mine >= 0x7f800000u) mine = 0u;
+      if (above(__reduce_max_sync(kFull, mine)) > vref) {
+        // a row of zeros has the scale 1, however small the others are: it counts as 0
+        const unsigned char* values = smem + (warp * kS + stage) * Plan::kStage + Plan::kTile;
+        if (above(mine) > vref && row_is_zero<kRow>(values, my_key)) sc[kKeys + my_key] = mine = 0;
+        __syncwarp();
+        const uint32_t top = above(__reduce_max_sync(kFull, mine));
+        if (top > vref) {  // the sums so far become relative to the new one
+          shrink = exp2f(static_cast<float>(static_cast<int>(vref) - static_cast<int>(top)));
+          vref = top;
+        }
       }
       const float down = __uint_as_float((254 - vref) << 23);
 #pragma unroll

@@ -65,3 +65,22 @@ def test_infinite_values_under_small_weights(n, best, at, gap, dtype, variant):
         assert torch.all(got[..., 9] == float("inf")) and torch.all(got[..., 5] == float("-inf"))
         live = torch.tensor([i for i in range(D) if i not in (5, 9)], device=DEV)
         base.check(got[..., live], want[..., live], base.attention_limit(*clean, 1.0))
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Hq,D", [(4, 64), (4, 128), (12, 128), (4, 256), (12, 96)])
+def test_zero_rows_among_tiny_values(Hq, D, dtype, variant):
+    # a row of zeros has the scale 1, whatever the others' are; here those lie near 2^-38.
+    # fp16 is left out: the results are far below its smallest number
+    q, k, v = rows_of(5, Hq, 1, D, 300, dtype, 2)
+    v *= 1e-9
+    v[0, :, 7] = 0.0         # one in the middle of a tile
+    v[1, :, :40] = 0.0       # the first tiles whole
+    v[2, :, 250:] = 0.0      # the last ones
+    v[3, :, ::2] = 0.0       # every other
+    v[4, :, 1:] = 0.0        # all but one
+    ins = inputs(q, k, v, dtype, 1)
+    for n in (300, 40, 1):
+        ins[4].fill_(n)
+        base.check_paged(ins, variant)
