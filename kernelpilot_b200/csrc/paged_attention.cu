@@ -791,6 +791,10 @@ __device__ __forceinline__ bool tile_has_inf(const unsigned char* tile, int byte
   return __any_sync(kFull, __hisinf(__low2half(top)) != 0 || __hisinf(__high2half(top)) != 0);
 }
 
+// Queries of e4m3 products are held with the head's largest element at 2^14 to 2^15, the top
+// of fp16's range; the products' sums (2^15 x 448 x 256 at most) have room for it in fp32.
+constexpr uint32_t kQueryBits = 14;
+
 // Four e4m3 codes as two pairs of fp16, exactly.
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* lo, uint32_t* hi) {
   asm("{\n\t.reg .b16 l, h;\n\t"
@@ -861,12 +865,14 @@ constexpr uint32_t kBadRow = 0xfffffffeu;  // in a page outside the cache
 // weights' fragments over (movmatrix) and adds O^T += V^T P^T (elements x heads). The
 // weights enter as two 16-bit parts (split_weights), so that they carry 2^-15 of themselves
 // (bf16) or 2^-21 (fp16); the second product is a small part of the time that loading takes.
-// e4m3: codes become fp16 in registers, q is scaled by a power of two to [1, 2) (exact; fp32
-// queries as two fp16 parts, 2^-22 of the largest element and less) and the key's scale
-// multiplies its score. The value's scale multiplies the weight, relative to
-// the power of two above the largest scale that the warp has met, rows of zeros aside (the
-// running sums follow when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's full
-// fraction while its scale is above 2^-28 of the largest.
+// e4m3: codes become fp16 in registers, q is scaled by a power of two so that the head's
+// largest element lies in [2^14, 2^15), and the key's scale multiplies its score. A bf16
+// element is then exact down to 2^-31 of the largest, an fp16 one down to 2^-28, and off by
+// 2^-39 of the largest below that; fp32 queries enter as two fp16 parts, off by 2^-22 of the
+// element or by that 2^-39. The value's scale multiplies the weight, relative to the power of
+// two above the largest scale that the warp has met, rows of zeros aside (the running sums
+// follow when it grows): with the 2^14 that weights are held at, a weight of 1 keeps fp16's
+// full fraction while its scale is above 2^-28 of the largest.
 template <typename T, typename C, int DP, int NT>
 __global__ void __launch_bounds__(kSplitThreads)
 split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __restrict__ v_cache,
@@ -1012,10 +1018,13 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           }
           top = max(top, __shfl_xor_sync(kFull, top, 1));
           top = max(top, __shfl_xor_sync(kFull, top, 2));
-          // 2^-e and 2^e of the head's largest magnitude; 1 for zeros and what is not finite
+          // down: brings the head's largest magnitude, of exponent ex, to [2^kQueryBits,
+          // 2^(kQueryBits + 1)); up = 1 / down. Both stay normal numbers: what is smaller than
+          // 2^(kQueryBits - 126) is scaled by 2^126. A head that is not finite ends as NaN
           uint32_t ex = top >> 23;
-          ex = ex == 0 || ex == 255 ? 127 : ex > 253 ? 253 : ex;
-          const float down = __uint_as_float((254 - ex) << 23), up = __uint_as_float(ex << 23);
+          ex = ex == 255 ? 127 : max(ex, kQueryBits + 1u);
+          const float down = __uint_as_float((254 + kQueryBits - ex) << 23);
+          const float up = __uint_as_float((ex - kQueryBits) << 23);
 #pragma unroll
           for (int kk = 0; kk < kSteps; ++kk) {
             const T* e = reinterpret_cast<const T*>(&raw[kk]);

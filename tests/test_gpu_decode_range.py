@@ -3,6 +3,8 @@ reference."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -84,3 +86,34 @@ def test_zero_rows_among_tiny_values(Hq, D, dtype, variant):
     for n in (300, 40, 1):
         ins[4].fill_(n)
         base.check_paged(ins, variant)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype,ratio", [(torch.bfloat16, 12), (torch.bfloat16, 20),
+                                         (torch.bfloat16, 24), (torch.float16, 20),
+                                         (torch.float32, 20)], ids=str)
+@pytest.mark.parametrize("Hq,D", [(4, 64), (12, 128), (4, 256)])
+def test_queries_with_one_large_channel(Hq, D, dtype, ratio, variant):
+    # the large channel meets zeros in every key, so the scores are the other channels' alone.
+    # e4m3 products take q as fp16 with the head's largest element at 2^14: the smallest here,
+    # 2^29 below, lies at 2^-15 and keeps a bf16's eight bits (fp16: 2^25 below, eleven bits),
+    # so that 16-bit queries are exact; an fp32 one is off by 2^-25, half of fp16's smallest
+    # number, which is 2^-39 of the largest element
+    q, k, v = rows_of(3, Hq, 1, D, 200, dtype, 3)
+    low = 2.0 ** -8 if dtype == torch.float16 else 1.0
+    q.copy_(torch.clamp(q.float().abs(), min=0.05) * q.float().sign() * low)
+    q[..., 0] = low * 2.0 ** ratio
+    k[..., 0] = 0.0
+    ins = inputs(q, k, v, dtype, 1)
+    scale = 1.0 / (math.sqrt(D) * low)
+    lim = base.attention_limit(*ins, scale)
+    if dtype == torch.float32 and variant == 1:
+        # each of D channels off by 2^-39 of the largest element: the score by that times the
+        # sum of |k|, a weight by twice it
+        kk = sd._values(ins[1], ins[5], torch.arange(ins[1].shape[0], device=DEV)[:, None],
+                        torch.arange(16, device=DEV), torch.float64)
+        off = 2.0 ** (ratio - 39) * float(kk.abs().sum(-1).max()) * scale
+        lim = lim + 2 * off * float(v.abs().max())
+    got = base.run_paged(ins, variant, scale)
+    (want,) = sd.paged_attention_reference(*ins, scale)
+    base.check(got, want, lim)
