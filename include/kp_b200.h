@@ -229,6 +229,8 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * A score of NaN or +inf, or no score above -inf, makes the head's output NaN, as the
  * softmax does; a page outside the cache makes the sequence's heads NaN, a length past the
  * table is cut to it and a negative one is none (bit 2 either way).
+ * Values are summed before the division: with the largest weight 1, the sum of weights times
+ * |V| must stay below fp32's largest number. Weights below 2^-126 of the largest count as 0.
  * Value scales of an E4M3 cache must not be negative; those of one sequence may span 2^28
  * before weights lose bits to the largest. Rows of zeros do not count, whatever their scale.
  * Queries on an E4M3 cache (variant 1, D <= 128 for fp32) are exact down to 2^-28 of their

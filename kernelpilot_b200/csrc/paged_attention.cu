@@ -741,6 +741,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
+// fp16 weights are held times 2^14 (the maximum's weight is 16384): they keep their full
+// fraction down to 2^-28 of the largest and something down to 2^-38. bf16 has fp32's range, and
+// its weights are held as they are: 2^14 would bring sums of values from 2^114 on to infinity.
+template <typename M>
+constexpr float kWeightBits = std::is_same_v<M, __half> ? 14.f : 0.f;
+template <typename M>
+constexpr float kWeightUnit = std::is_same_v<M, __half> ? 0x1p-14f : 1.f;
+
 // The smallest fp16 number.
 constexpr float kHalfTiny = 0x1p-24f;
 
@@ -750,6 +758,7 @@ constexpr float kHalfTiny = 0x1p-24f;
 // value times the two is then an infinity, not infinity * 0 or the difference of two.
 template <typename M, bool kCut>
 __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* rest) {
+  constexpr float kTiny = std::is_same_v<M, __half> ? kHalfTiny : 0x1p-120f;
   uint32_t hi;
   float2 f;
   if constexpr (std::is_same_v<M, __half>) {
@@ -762,8 +771,8 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
   }
   float rx = x - f.x, ry = y - f.y;
   if constexpr (kCut) {
-    rx = fmaxf(rx, fminf(x, kHalfTiny));
-    ry = fmaxf(ry, fminf(y, kHalfTiny));
+    rx = fmaxf(rx, fminf(x, kTiny));
+    ry = fmaxf(ry, fminf(y, kTiny));
   }
   if constexpr (std::is_same_v<M, __half>) {
     const __half2 v = __floats2half2_rn(rx, ry);
@@ -774,10 +783,6 @@ __device__ __forceinline__ uint32_t split_weights(float x, float y, uint32_t* re
   }
   return hi;
 }
-
-// Weights are held times 2^14 (the maximum's weight is 16384): fp16 then keeps its full
-// fraction down to 2^-28 of the largest weight and something down to 2^-38.
-constexpr float kWeightBits = 14.f;
 
 // Whether a tile of `bytes` bytes of fp16 holds an infinity (same answer in every lane).
 __device__ __forceinline__ bool tile_has_inf(const unsigned char* tile, int bytes) {
@@ -1160,7 +1165,7 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
         for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits));
+            w[j][h][i] = ex2f(w[j][h][i] - (base - kWeightBits<M>));
             sum += w[j][h][i];
             if constexpr (kQuant) w[j][h][i] *= vs[j][h];
           }
@@ -1271,21 +1276,22 @@ split_mma(const T* __restrict__ q, const C* __restrict__ k_cache, const C* __res
           for (int off = 4; off < kWarp; off <<= 1) sum += __shfl_xor_sync(kFull, sum, off);
           const int h = nt * 8 + 2 * t + i;
           if (first + h < sp.group) {
-            // values of e4m3 rows are relative to 2^(vref - 127)
-            float f = kQuant ? __uint_as_float(vref << 23) : 1.f;
-            if (whole) f /= sum;
+            // out of the weights' units, and of 2^(vref - 127) for e4m3 values: one after the
+            // other, since the product of the two may leave fp32's range
+            const float f = whole ? 1.f / sum : kWeightUnit<M>;
+            const float vf = kQuant ? __uint_as_float(vref << 23) : 1.f;
             T* out = o + (p.b * sh.q_heads + hk * sp.group + first + h) * dim;
             float* part = partial_at(sp, worker, slot, h);
             if (!whole && r == 0) {
               part[DP] = m[nt][i];
-              part[DP + 1] = sum;
+              part[DP + 1] = sum * f;
             }
 #pragma unroll
             for (int kk = 0; kk < kSteps; ++kk) {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 const int d = kk * 16 + (kQuant ? 2 * r + j : r + 8 * j);
-                const float v = acc[nt][kk][2 * j + i] * f;
+                const float v = acc[nt][kk][2 * j + i] * f * vf;
                 if (!whole) part[d] = v;
                 else if (d < dim) out[d] = from_f<T>(v);
               }

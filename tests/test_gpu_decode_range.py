@@ -117,3 +117,19 @@ def test_queries_with_one_large_channel(Hq, D, dtype, ratio, variant):
     got = base.run_paged(ins, variant, scale)
     (want,) = sd.paged_attention_reference(*ins, scale)
     base.check(got, want, lim)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("size", [115, -118])
+def test_very_large_and_very_small_values(size, e4m3, dtype, variant):
+    # 700 weights of at most 1 over values of up to 6 * 2^115 sum to less than 2^128; the small
+    # ones are far above fp32's smallest normal number, 2^-126
+    for Hq, D in ((4, 64), (4, 128), (12, 128), (4, 256)):
+        q, k, v = rows_of(2, Hq, 1, D, 700, dtype, 4)
+        v *= 2.0 ** size
+        ins = inputs(q, k, v, dtype, e4m3)
+        for n in (700, 16):  # joined from parts, and not
+            ins[4].fill_(n)
+            base.check_paged(ins, variant)
