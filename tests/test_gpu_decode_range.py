@@ -133,3 +133,43 @@ def test_very_large_and_very_small_values(size, e4m3, dtype, variant):
         for n in (700, 16):  # joined from parts, and not
             ins[4].fill_(n)
             base.check_paged(ins, variant)
+
+
+def weight_error(dtype, e4m3, variant):
+    """What a weight may be off by beside fp32's roundings, relative to itself: where weights
+    enter the products as two 16-bit parts, what the two leave. bf16: the first is cut to 8
+    bits (2^-7 left), the second rounded to 2^-8 of that. fp16 values: cut to 11 bits (2^-10),
+    2^-11 of that; e4m3 values, as fp16: rounded (2^-11), 2^-11 of that."""
+    if variant == 0 or (dtype == torch.float32 and not e4m3):
+        return 0.0
+    if e4m3:
+        return 2.0 ** -22
+    return 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -21
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", base.DTYPES)
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("n", [2, 3, 5])
+def test_weights_keep_the_bits_of_their_path(n, e4m3, dtype, variant):
+    # one channel of q and k makes the scores, of at most 4 and exact but for the roundings of
+    # one product (16-bit q) or of q's two fp16 parts (2^-22, fp32 q on e4m3), the scale and
+    # the change to powers of two: 4 * 2^-24 of 4 and 2^-22 of 4. The maximum's subtraction is
+    # off by 2^-24 of 4 too, 2^x by 2^-22 (twice: above and below the division); up to n + 6
+    # roundings of the sums, the division and the products, and 2^-23 for each of the four tensor
+    # core products, whose sums are cut
+    B, Hq, D = 32, 4, 64
+    q, k, v = rows_of(B, Hq, 1, D, n, dtype, 5)
+    top = 1.0 + torch.rand(B, Hq, generator=base.generator(6), device=DEV)
+    q.zero_()[..., 0] = top.to(dtype)
+    k.zero_()[..., 0] = torch.randint(0, 16, k.shape[:3], generator=base.generator(7),
+                                      device=DEV) / 8.0
+    ins = inputs(q, k, v, dtype, e4m3)
+    got = base.run_paged(ins, variant, 1.0)
+    (want,) = sd.paged_attention_reference(*ins, 1.0)
+    # sum of w |v| per output element
+    absolute = (*ins[:2], ins[2].float().abs().to(ins[2].dtype), *ins[3:])
+    (av,) = sd.paged_attention_reference(*absolute, 1.0)
+    score = 4 * (5 * base.U24 + (2.0 ** -22 if e4m3 and dtype == torch.float32 else 0.0))
+    rel = 2 * score + 2 * 2.0 ** -22 + (n + 14) * base.U24 + 2 * weight_error(dtype, e4m3, variant)
+    base.check(got, want, rel * av)
