@@ -235,8 +235,9 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * before weights lose bits to the largest. Rows of zeros do not count, whatever their scale.
  * Queries on an E4M3 cache (variant 1, D <= 128 for fp32) are exact down to 2^-28 of their
  * head's largest element and off by 2^-39 of it below; fp32 ones by 2^-22 of the element too.
- * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size),
- * asked for on the device of the call, 16-byte aligned, the call's own until it has run. */
+ * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size; 0
+ * for sizes that the call refuses), asked for on the device of the call, 16-byte aligned, the
+ * call's own until it has run. */
 size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,
                                            int64_t D, int64_t max_len);
 int kpb_paged_attention(int variant, int dtype, int cache_dtype, const void* q,

@@ -577,7 +577,7 @@ static int check_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
 
 size_t kpb_paged_attention_workspace_bytes(int variant, int64_t B, int64_t Hq, int64_t Hkv,
                                            int64_t D, int64_t max_len) {
-  if (variant < 0 || variant >= kpb_num_variants("paged_attention") || max_len < 0 ||
+  if (variant < 0 || variant >= kpb_num_variants("paged_attention") || !size_ok(max_len) ||
       check_paged(B, Hq, Hkv, D) != KPB_OK || B == 0 || Hq == 0)
     return 0;
   return paged_attention_workspace_bytes(variant, B, Hq, Hkv, D, max_len);

@@ -1,9 +1,11 @@
 """Host-side bounds of the decode operators, without a GPU: which notes on shared rows the
-attention's second kernel follows."""
+attention's second kernel follows, and the sizes that its workspace query takes."""
 
 import subprocess
 
-from kernelpilot_b200 import build
+import pytest
+
+from kernelpilot_b200 import build, ext
 
 PROGRAM = r"""
 #include <cstdio>
@@ -32,3 +34,14 @@ def test_no_note_leads_past_the_partials(tmp_path):
     for (first, count, workers), got in zip(cases, out, strict=True):
         want = first >= 0 and count >= 0 and first // 2 < workers and first // 2 + count <= workers
         assert got == str(int(want)), (first, count, workers)
+
+
+@pytest.mark.parametrize("B", [1, 4, 1 << 20])
+def test_workspace_query_of_lengths_past_the_limit(B):
+    # max_pages * page_size must be below 2^31; the query answers 0 for what the call refuses,
+    # and never less for a longer table than for a shorter one
+    query = ext.capi().kpb_paged_attention_workspace_bytes
+    sizes = [query(1, B, 32, 8, 128, n) for n in (1, 16, 1000, 1 << 20, (1 << 31) - 1)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    for n in (1 << 31, 1 << 40, (1 << 63) - 1, -1):
+        assert query(1, B, 32, 8, 128, n) == 0
