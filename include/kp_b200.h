@@ -170,7 +170,8 @@ int kpb_attention_causal(int variant, int dtype, const void* q, const void* k,
  * (2i, 2i + 1) if `interleaved`. cos_sin is fp32 (max_pos, rot): rot/2 cosines then rot/2
  * sines per position. q is (T, Hq, D) and k (T, Hkv, D), the heads of a token contiguous
  * and tokens q_stride / k_stride elements apart (slices of a fused projection); q_out and
- * k_out are contiguous. fp32 until one rounding to the dtype. */
+ * k_out are contiguous and overlap no input. fp32 until one rounding to the dtype: a row's sum
+ * of squares must stay below fp32's largest number. */
 int kpb_qk_norm_rope(int variant, int dtype, const void* q, const void* k, const void* q_weight,
                      const void* k_weight, const float* cos_sin, const int64_t* positions,
                      void* q_out, void* k_out, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
@@ -179,8 +180,8 @@ int kpb_qk_norm_rope(int variant, int dtype, const void* q, const void* k, const
 
 /* Its gradient: from grad_q, grad_k (the gradients of q_out, k_out) and the forward's
  * inputs, dq (T, Hq, D), dk (T, Hkv, D) contiguous and dq_weight, dk_weight (D), every one
- * overwritten. The weight gradients are summed over all rows in fp32 in a fixed order (the
- * same bits every time on one kind of GPU). workspace: kpb_qk_norm_rope_backward_
+ * overwritten; no output overlaps an input. The weight gradients are summed over all rows in
+ * fp32 in a fixed order (the same bits every time on one kind of GPU). workspace: kpb_qk_norm_rope_backward_
  * workspace_bytes() bytes, 16-byte aligned, the call's own until it has run. */
 size_t kpb_qk_norm_rope_backward_workspace_bytes(int64_t T, int64_t Hq, int64_t Hkv, int64_t D);
 int kpb_qk_norm_rope_backward(int variant, int dtype, const void* grad_q, const void* grad_k,
@@ -230,8 +231,10 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * softmax does; a page outside the cache makes the sequence's heads NaN, a length past the
  * table is cut to it and a negative one is none (bit 2 either way).
  * Values are summed before the division: with the largest weight 1, the sum of weights times
- * |V| must stay below fp32's largest number. Weights below 2^-126 of the largest count as 0.
- * Value scales of an E4M3 cache must not be negative; those of one sequence may span 2^28
+ * |V| must stay below fp32's largest number. Weights below 2^-126 of the largest may count as
+ * 0. Variant 1 takes 16-bit weights in two parts: off by 2^-15 of themselves on bf16 caches, by
+ * 2^-21 of themselves and up to 2^-38 of the largest on fp16 ones.
+ * Value scales of an E4M3 cache must be NaN, or finite and not negative; those of one sequence may span 2^28
  * before weights lose bits to the largest. Rows of zeros do not count, whatever their scale.
  * Queries on an E4M3 cache (variant 1, D <= 128 for fp32) are exact down to 2^-28 of their
  * head's largest element and off by 2^-39 of it below; fp32 ones by 2^-22 of the element too.
