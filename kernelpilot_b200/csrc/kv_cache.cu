@@ -16,8 +16,9 @@
 //
 // Measured on B200 (6464 GB/s copy), 8 heads of 128, pages of 16: e4m3 write of 32768 bf16
 // tokens 35 us (204 MB; 31.5 us at copy bandwidth), variant 0 125; bf16 read of 65536 tokens
-// 83 us (537 MB; 83), variant 0 163; e4m3 read of 5001 tokens 5.7 us (31 MB; 4.8). With one
-// vector a lane and unpacked maxima the write took 54 us, the reads 89 and 7.4.
+// 83 us (537 MB; 83), variant 0 163; e4m3 read of 5001 tokens 6.2 us (31 MB; 4.8); plain bf16
+// write of 32768 tokens 43.5 us (269 MB; 41.6). With one vector a lane and unpacked maxima the
+// e4m3 write took 54 us, the reads 89 and 7.4.
 #include "kp_kv_cache.cuh"
 
 namespace kpb {

@@ -32,10 +32,10 @@
 // conversion to fp16 and the warps' latency as much. Measured on B200 (6464 GB/s copy), head
 // dim 128, 8 key heads, ragged lengths:
 //   64 sequences up to 8192 keys, bf16, 32 query heads    174 us (1065 MB; 165 at that rate)
-//   32 sequences up to 16384 keys, e4m3, 64 query heads   101 us (549 MB; 85)
+//   32 sequences up to 16384 keys, e4m3, 64 query heads   103 us (549 MB; 85)
 //   64 sequences up to 4096 keys, fp32, 32 query heads    184 us (1066 MB; 165)
-//   2 sequences up to 32768 keys, fp16, 32 heads of 64     76 us (434 MB; 67)
-//   one sequence of 1037 keys, bf16, 32 query heads       10.4 us, 3 of them the join's launch
+//   2 sequences up to 32768 keys, fp16, 32 heads of 64     77 us (434 MB; 67)
+//   one sequence of 1037 keys, bf16, 32 query heads       11.0 us, 3 of them the join's launch
 // variant 0 takes 4764, 9193, -, 12317 and 274 us on the same calls.
 #include <algorithm>
 

@@ -29,7 +29,10 @@
 //
 // Measured on B200 (6464 GB/s copy), 16384 tokens, 32 + 8 heads of 128, bf16: forward 59 us
 // (344 MB; 53 us at copy bandwidth), variant 0 265; backward 95 us (512 MB; 79), variant 0
-// 955. 64 tokens: forward 2.3 us.
+// 955. 64 tokens: forward 2.9 us. Other shapes are further off, variant 1's turns and lanes
+// being padded: heads of 80 and 96 elements take 8 lanes for 5 and 6 pairs (32768 tokens, 24 + 8
+// heads: 86 us for 54 at copy bandwidth, 88 for 64), and a turn costs four heads where it has
+// one (4 + 1 heads of 128: 26 us for 16).
 #include <algorithm>
 
 #include "kp_kv_cache.cuh"
