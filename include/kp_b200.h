@@ -234,8 +234,9 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * |V| must stay below fp32's largest number. Weights below 2^-126 of the largest may count as
  * 0. Variant 1 takes 16-bit weights in two parts: off by 2^-15 of themselves on bf16 caches, by
  * 2^-21 of themselves and up to 2^-38 of the largest on fp16 ones.
- * Value scales of an E4M3 cache must be NaN, or finite and not negative; those of one sequence may span 2^28
- * before weights lose bits to the largest. Rows of zeros do not count, whatever their scale.
+ * Value scales of an E4M3 cache must be NaN, or finite and not negative; those of one sequence
+ * may span 2^28 before weights lose bits to the largest. Rows of zeros do not count, whatever
+ * their scale.
  * Queries on an E4M3 cache (variant 1, D <= 128 for fp32) are exact down to 2^-28 of their
  * head's largest element and off by 2^-39 of it below; fp32 ones by 2^-22 of the element too.
  * workspace: kpb_paged_attention_workspace_bytes() bytes (max_len = max_pages * page_size; 0
