@@ -230,6 +230,8 @@ int kpb_kv_cache_read(int variant, int dtype, int cache_dtype, const void* k_cac
  * A score of NaN or +inf, or no score above -inf, makes the head's output NaN, as the
  * softmax does; a page outside the cache makes the sequence's heads NaN, a length past the
  * table is cut to it and a negative one is none (bit 2 either way).
+ * q . K[j] is summed before the scale (16-bit caches, variant 1) or after it, and must stay
+ * within fp32 there.
  * Values are summed before the division: with the largest weight 1, the sum of weights times
  * |V| must stay below fp32's largest number. Weights below 2^-126 of the largest may count as
  * 0. Variant 1 takes 16-bit weights in two parts: off by 2^-15 of themselves on bf16 caches, by

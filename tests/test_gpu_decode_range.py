@@ -173,3 +173,41 @@ def test_weights_keep_the_bits_of_their_path(n, e4m3, dtype, variant):
     score = 4 * (5 * base.U24 + (2.0 ** -22 if e4m3 and dtype == torch.float32 else 0.0))
     rel = 2 * score + 2 * 2.0 ** -22 + (n + 14) * base.U24 + 2 * weight_error(dtype, e4m3, variant)
     base.check(got, want, rel * av)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("size", [124, 60, -60, -110, -122])
+def test_queries_of_any_size(size, e4m3, dtype, variant):
+    # the score's scale brings them back; the smallest elements are fp32's subnormals (a bf16's
+    # too), exact in the inputs
+    q, k, v = rows_of(2, 4, 1, 64, 90, dtype, 8)
+    ins = inputs((q.float() * 2.0 ** size).to(dtype), k, v, dtype, e4m3)
+    if size == 124 and dtype == torch.bfloat16 and not e4m3 and variant == 1:
+        # outside what kp_b200.h allows: 16-bit products are summed before the scale, and sums of
+        # 64 products of values near 2^124 and 1 pass fp32's largest number
+        sums = ins[0].double().abs() @ ins[1].double().abs().amax(0)[0].transpose(0, 1)
+        assert float(sums.max()) > torch.finfo(torch.float32).max
+        return
+    base.check_paged(ins, variant, scale=2.0 ** -size / 8)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", base.DTYPES)
+def test_e4m3_rows_and_queries_that_are_not_finite(dtype, variant):
+    # a key or value row that was not finite has the scale NaN: its sequence's heads are NaN; so
+    # is a head whose query holds an infinity or NaN, and no other
+    q, k, v = rows_of(4, 4, 1, 64, 90, dtype, 9)
+    q[2, 1, 3], q[2, 2, 60] = float("inf"), float("nan")
+    k[0, 0, 50, 7] = float("inf")
+    v[1, 0, 3, 9] = float("nan")
+    ins = inputs(q, k, v, dtype, 1)
+    got = base.run_paged(ins, variant)
+    (want,) = sd.paged_attention_reference(*ins)
+    assert torch.isnan(got[:2]).all() and torch.isnan(want[:2]).all()
+    assert torch.isnan(got[2, 1:3]).all() and torch.isnan(want[2, 1:3]).all()
+    clean = (q.nan_to_num(posinf=0.0), *ins[1:])
+    lim = base.attention_limit(*clean)
+    for at in ((2, slice(0, 1)), (2, slice(3, 4)), (3, slice(0, 4))):
+        base.check(got[at], want[at], lim[at])
